@@ -186,6 +186,94 @@ int nvfp4_gemv_call(const nvfp4_gemv_args* args);
 int nvfp4_gemm_call(const nvfp4_gemm_args* args);
 int nvfp4_dual_gemm_call(const nvfp4_gemm_args* args);
 
+/* ------------------------------------------------------------------------
+ * MXFP4 (the OCP microscaling format) and products over experts.  No
+ * counterpart in the reference.
+ *
+ *   codes  : e2m1, rows x K/2 bytes without gaps, even K index in the low nibble
+ *   scales : e8m0, one byte per 32 elements (2^(code - 127), 255 = NaN), in the
+ *            128x4-blocked order above with K/32 columns: the scales of
+ *            128 rows x 128 columns of K are 512 contiguous bytes, byte (i, j)
+ *            of them at (i%32)*16 + (i/32)*4 + j; the blocks of a matrix go
+ *            along K (ceil(K/128) of them) and then down the rows.  Rows past
+ *            the last are padding; so are columns past K/32, which the
+ *            quantiser writes as 0 and the products ignore.
+ *
+ * Rows sorted by expert: offsets[experts + 1] (device memory) gives expert e
+ * the rows offsets[e] .. offsets[e+1]-1.  The codes of all rows follow one
+ * another; the scales of each expert begin a new 128-row block, so
+ * min(rows, experts) + rows/128 blocks hold them whatever the offsets.  Rows
+ * behind offsets[experts] belong to nobody: what reads rows skips them, what
+ * writes rows of values writes zeros there, and the quantiser leaves them as
+ * they were.  At most 1024 experts. */
+
+/* x (fp16, bf16 or fp32: dtype 0, 1, 2) and its MXFP4 form.  x has `experts`
+ * matrices of `rows` rows of K elements (x_estride, x_rstride elements apart),
+ * each with its own scale blocks; K % 32 == 0.
+ *   offsets != NULL : `rows` rows sorted by expert, in all.
+ *   slots != NULL   : (with offsets; quantiser only) `rows` tokens; token t is
+ *                     quantised once and written to the sorted rows
+ *                     slots[t*top] .. slots[t*top + top-1] (negative: to none).
+ *   columns != 0    : (quantiser only, one matrix) blocks down the columns:
+ *                     the codes and scales of the transpose, K rows of `rows`
+ *                     elements padded with zeros to a multiple of 32 (any K).
+ * Per block of 32: code = max(floor(log2(amax)) - 2 + 127, 0), values
+ * e2m1_rn_satfinite(x * 2^(127 - code)); code 255 and zero values where the
+ * block holds a NaN or an infinity.
+ * nvfp4_mx_dequantize writes values of type dtype to x (contiguous, 16-byte aligned). */
+typedef struct {
+  const void* x;
+  void* packed;
+  void* scales;
+  const int32_t* offsets;
+  const int32_t* slots;
+  int32_t dtype, rows, K, experts, top, columns;
+  int64_t x_rstride, x_estride;
+  void* stream;
+} nvfp4_mx_quant_args;
+
+int nvfp4_mx_quantize(const nvfp4_mx_quant_args* args);
+int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* args);
+
+/* Sorts n slots by expert, stably: ids[n] (int32 or int64: id_bytes 4, 8);
+ * an id outside 0 .. experts-1 is not routed.
+ *   order[n]           the slot of each sorted row, -1 behind the last
+ *   slots[n]           the sorted row of each slot, -1 where it is not routed
+ *   offsets[experts+1] the first row of each expert, and the number of rows
+ * The workspace (nvfp4_moe_sort_workspace bytes, 0 for short lists; -1 for bad
+ * arguments) is the caller's and needs no preparation. */
+int64_t nvfp4_moe_sort_workspace(int n, int experts);
+int nvfp4_moe_sort(const void* ids, int id_bytes, int n, int experts, int32_t* order, int32_t* slots, int32_t* offsets,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows between tokens and experts; slots [tokens][top], offsets as nvfp4_moe_sort
+ * gives them, rows = tokens * top, all values of type dtype, sums in fp32:
+ *   gather            out[rows][hidden]   = in[token]                  (in: x)
+ *   gather_backward   out[tokens][hidden] = sum of in[row]             (in: dxs)
+ *   combine           out[tokens][hidden] = sum of weights * in[row]   (in: ys)
+ *   combine_backward  out[rows][hidden]   = weights * grad[token],
+ *                     dweights[tokens][top] = <grad[token], in[row]>   (in: ys, grad: dy)
+ * Rows of `in` and `grad` are in_stride, grad_stride elements apart; out is
+ * contiguous.  weights and dweights are fp32 [tokens][top]; a slot that is not
+ * routed adds nothing and gets dweights 0. */
+typedef struct {
+  const void* in;
+  const void* grad;
+  const float* weights;
+  void* out;
+  float* dweights;
+  const int32_t* slots;
+  const int32_t* offsets;
+  int32_t dtype, tokens, top, hidden, experts, reserved;
+  int64_t in_stride, grad_stride;
+  void* stream;
+} nvfp4_moe_args;
+
+int nvfp4_moe_gather(const nvfp4_moe_args* args);
+int nvfp4_moe_gather_backward(const nvfp4_moe_args* args);
+int nvfp4_moe_combine(const nvfp4_moe_args* args);
+int nvfp4_moe_combine_backward(const nvfp4_moe_args* args);
+
 #ifdef __cplusplus
 }
 #endif

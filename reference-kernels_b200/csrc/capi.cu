@@ -416,6 +416,131 @@ NVFP4_API int nvfp4_scales_from_blocked(const void* blk, void* plain, int rows, 
                       blk_lstride, stream);
 }
 
+// ------------------------------------------------------------------ MXFP4 and experts
+constexpr int kMaxExpertsApi = 1024;
+
+static int64_t dtype_size(int dtype) { return dtype == 2 ? 4 : 2; }
+
+// The checks that the quantiser and the dequantiser share; fills `a`.
+static int mx_quant_args(const char* name, const nvfp4_mx_quant_args* x, bool quantize, MxQuantArgs& a) {
+  if (!x) return fail(NVFP4_ERR_NULL, "%s: null argument block", name);
+  if (x->dtype < 0 || x->dtype > 2) return fail(NVFP4_ERR_SHAPE, "%s: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)", name);
+  if (x->rows < 0 || x->K <= 0 || x->experts < 1)
+    return fail(NVFP4_ERR_SHAPE, "%s: rows=%d must not be negative, K=%d and experts=%d must be positive", name, x->rows,
+                x->K, x->experts);
+  if (x->columns && (!quantize || x->offsets || x->slots || x->experts != 1))
+    return fail(NVFP4_ERR_SHAPE, "%s: blocks down the columns are for one matrix to be quantised", name);
+  if (!x->columns && x->K % 32) return fail(NVFP4_ERR_SHAPE, "%s: K=%d must be a multiple of 32", name, x->K);
+  if (x->offsets && x->experts > kMaxExpertsApi)
+    return fail(NVFP4_ERR_SHAPE, "%s: %d experts, at most %d", name, x->experts, kMaxExpertsApi);
+  if (x->slots && (!quantize || !x->offsets || x->top < 0))
+    return fail(NVFP4_ERR_SHAPE, "%s: slots need offsets and top >= 0", name);
+  const int64_t rows = x->offsets ? x->rows : static_cast<int64_t>(x->rows) * x->experts;
+  const int64_t units = rows * ((static_cast<int64_t>(x->K) + 511) / 512);
+  const int64_t sorted = x->slots ? static_cast<int64_t>(x->rows) * x->top : rows;
+  if (rows > INT32_MAX || units > INT32_MAX || sorted > INT32_MAX || (x->columns && x->rows > 65535 * 256))
+    return fail(NVFP4_ERR_SHAPE, "%s: too many rows", name);
+  if (rows > 0 && sorted > 0) {
+    if (!x->x || !x->packed || !x->scales) return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
+    if (!aligned(x->x, quantize ? dtype_size(x->dtype) : 16) || !aligned(x->packed, 16) || !aligned(x->scales, 16) ||
+        !aligned(x->offsets, 4) || !aligned(x->slots, 4))
+      return fail(NVFP4_ERR_ALIGN, "%s: codes and scales need 16-byte alignment, x that of its type%s", name,
+                  quantize ? "" : " and 16 bytes");
+  }
+  a = MxQuantArgs{x->x,       x->packed, x->scales, x->offsets, x->slots, x->dtype, static_cast<int>(rows), x->K, x->rows,
+                  x->experts, x->top,    static_cast<int>(sorted), x->columns, x->x_rstride, x->x_estride};
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_mx_quantize(const nvfp4_mx_quant_args* x) {
+  MxQuantArgs a;
+  const int rc = mx_quant_args("nvfp4_mx_quantize", x, true, a);
+  if (rc) return rc;
+  if (a.rows == 0 || a.sorted_rows == 0) return NVFP4_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "nvfp4_mx_quantize: no CUDA device");
+  const cudaError_t e = launch_mx_quantize(a, num_sms_of(dev), static_cast<cudaStream_t>(x->stream));
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "nvfp4_mx_quantize: %s", cudaGetErrorString(e));
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* x) {
+  MxQuantArgs a;
+  const int rc = mx_quant_args("nvfp4_mx_dequantize", x, false, a);
+  if (rc) return rc;
+  if (a.rows == 0) return NVFP4_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "nvfp4_mx_dequantize: no CUDA device");
+  const cudaError_t e = launch_mx_dequantize(a, num_sms_of(dev), static_cast<cudaStream_t>(x->stream));
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "nvfp4_mx_dequantize: %s", cudaGetErrorString(e));
+  return NVFP4_OK;
+}
+
+NVFP4_API int64_t nvfp4_moe_sort_workspace(int n, int experts) {
+  int dev = 0;
+  if (n < 0 || experts < 1 || experts > kMaxExpertsApi || cudaGetDevice(&dev) != cudaSuccess) return -1;
+  return static_cast<int64_t>(moe_sort_workspace_bytes(n, experts, num_sms_of(dev)));
+}
+
+NVFP4_API int nvfp4_moe_sort(const void* ids, int id_bytes, int n, int experts, int32_t* order, int32_t* slots,
+                             int32_t* offsets, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (id_bytes != 4 && id_bytes != 8) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: ids must have 4 or 8 bytes");
+  if (n < 0) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: n=%d must not be negative", n);
+  if (experts < 1 || experts > kMaxExpertsApi)
+    return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: experts=%d must be 1 to %d", experts, kMaxExpertsApi);
+  if (!offsets || (n && (!ids || !order || !slots))) return fail(NVFP4_ERR_NULL, "nvfp4_moe_sort: null pointer");
+  if (!aligned(ids, id_bytes) || !aligned(order, 4) || !aligned(slots, 4) || !aligned(offsets, 4) ||
+      !aligned(workspace, 4))
+    return fail(NVFP4_ERR_ALIGN, "nvfp4_moe_sort: every pointer needs its type's alignment");
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "nvfp4_moe_sort: no CUDA device");
+  const size_t need = moe_sort_workspace_bytes(n, experts, num_sms_of(dev));
+  if (need && (!workspace || workspace_bytes < static_cast<int64_t>(need)))
+    return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: the workspace needs %zu bytes", need);
+  MoeSortArgs a{ids, id_bytes, n, experts, order, slots, offsets, static_cast<int*>(workspace), 0};
+  const cudaError_t e = launch_moe_sort(a, num_sms_of(dev), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_sort: %s", cudaGetErrorString(e));
+  return NVFP4_OK;
+}
+
+static int moe_rows(const char* name, MoeRowOp op, const nvfp4_moe_args* x) {
+  if (!x) return fail(NVFP4_ERR_NULL, "%s: null argument block", name);
+  if (x->dtype < 0 || x->dtype > 2) return fail(NVFP4_ERR_SHAPE, "%s: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)", name);
+  if (x->tokens < 0 || x->top < 0 || x->hidden < 0 || x->experts < 1 || x->experts > kMaxExpertsApi)
+    return fail(NVFP4_ERR_SHAPE, "%s: tokens, top and hidden must not be negative, experts=%d must be 1 to %d", name,
+                x->experts, kMaxExpertsApi);
+  if (static_cast<int64_t>(x->tokens) * x->top > INT32_MAX) return fail(NVFP4_ERR_SHAPE, "%s: too many rows", name);
+  const bool weighted = op == kMoeCombine || op == kMoeCombineBackward;
+  const bool sorted_out = op == kMoeGather || op == kMoeCombineBackward;
+  const bool any = x->tokens && x->hidden;   // something to write by token
+  const bool rows = x->tokens && x->top;     // something to read or write by row
+  if ((any && !x->out && !(sorted_out && !rows)) || (any && rows && !x->in) || (rows && !x->slots) ||
+      (rows && sorted_out && !x->offsets) || (rows && weighted && !x->weights) ||
+      (rows && op == kMoeCombineBackward && (!x->dweights || (any && !x->grad))))
+    return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
+  const int64_t size = dtype_size(x->dtype);
+  if (!aligned(x->in, size) || !aligned(x->out, size) || !aligned(x->grad, size) || !aligned(x->slots, 4) ||
+      !aligned(x->offsets, 4) || !aligned(x->weights, 4) || !aligned(x->dweights, 4))
+    return fail(NVFP4_ERR_ALIGN, "%s: every pointer needs its type's alignment", name);
+  if (!x->tokens || (!x->hidden && op != kMoeCombineBackward) || (sorted_out && !x->top)) return NVFP4_OK;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "%s: no CUDA device", name);
+  MoeRowArgs a{x->in,    x->grad, x->weights, x->out,    x->dweights, x->slots,     x->offsets,
+               x->dtype, x->tokens, x->top,   x->hidden, x->experts,  x->in_stride, x->grad_stride};
+  const cudaError_t e = launch_moe_rows(op, a, num_sms_of(dev), static_cast<cudaStream_t>(x->stream));
+  if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_moe_gather(const nvfp4_moe_args* x) { return moe_rows("nvfp4_moe_gather", kMoeGather, x); }
+NVFP4_API int nvfp4_moe_gather_backward(const nvfp4_moe_args* x) {
+  return moe_rows("nvfp4_moe_gather_backward", kMoeGatherBackward, x);
+}
+NVFP4_API int nvfp4_moe_combine(const nvfp4_moe_args* x) { return moe_rows("nvfp4_moe_combine", kMoeCombine, x); }
+NVFP4_API int nvfp4_moe_combine_backward(const nvfp4_moe_args* x) {
+  return moe_rows("nvfp4_moe_combine_backward", kMoeCombineBackward, x);
+}
+
 // Packed-argument forms (include/nvfp4_b200.h): the same calls, one pointer.
 NVFP4_API int nvfp4_gemv_call(const nvfp4_gemv_args* x) {
   if (!x) return fail(NVFP4_ERR_NULL, "nvfp4_gemv_call: null argument block");

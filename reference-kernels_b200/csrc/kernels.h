@@ -141,4 +141,45 @@ struct ScaleLayoutArgs {
 };
 cudaError_t launch_scale_layout(const ScaleLayoutArgs& a, bool to_blocked, int num_sms, cudaStream_t stream);
 
+// MXFP4 quantiser and its reverse (mx_quant.cu).
+struct MxQuantArgs {
+  const void* x;  // fp16 (dtype 0), bf16 (1) or fp32 (2); the dequantiser's output
+  void* packed;
+  void* scales;
+  const int* offsets;  // rows sorted by expert (or null)
+  const int* slots;    // tokens to their sorted rows, [rows][top] (or null)
+  int dtype, rows, K;  // rows: all matrices' together; K: columns of x
+  int rows_per;        // rows of one matrix (offsets and slots null)
+  int experts, top;
+  int sorted_rows;     // rows of packed where offsets are given
+  int columns;         // blocks down the columns, result transposed
+  int64_t x_rstride, x_estride;  // elements
+};
+cudaError_t launch_mx_quantize(const MxQuantArgs& a, int num_sms, cudaStream_t stream);
+cudaError_t launch_mx_dequantize(const MxQuantArgs& a, int num_sms, cudaStream_t stream);
+
+// Tokens sorted by expert and back (moe.cu).
+struct MoeSortArgs {
+  const void* ids;  // [slots_n], int32 or int64 (id_bytes)
+  int id_bytes, slots_n, experts;
+  int *order, *slots, *offsets;
+  int* counts;  // workspace of moe_sort_workspace_bytes
+  int run;      // slots per CTA (set by the launcher)
+};
+size_t moe_sort_workspace_bytes(int n, int experts, int num_sms);
+cudaError_t launch_moe_sort(MoeSortArgs a, int num_sms, cudaStream_t stream);
+
+enum MoeRowOp { kMoeGather, kMoeGatherBackward, kMoeCombine, kMoeCombineBackward };
+struct MoeRowArgs {
+  const void* in;        // x, dxs, ys, ys
+  const void* grad;      // dy (combine_backward)
+  const float* weights;  // [tokens][top]
+  void* out;             // xs, dx, y, dys
+  float* dweights;       // [tokens][top]
+  const int *slots, *offsets;
+  int dtype, tokens, top, hidden, experts;
+  int64_t in_stride, grad_stride;  // elements
+};
+cudaError_t launch_moe_rows(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStream_t stream);
+
 }  // namespace nvfp4

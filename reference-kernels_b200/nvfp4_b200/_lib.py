@@ -28,6 +28,14 @@ EXPORTS = (
     "nvfp4_gemv_call",
     "nvfp4_gemm_call",
     "nvfp4_dual_gemm_call",
+    "nvfp4_mx_quantize",
+    "nvfp4_mx_dequantize",
+    "nvfp4_moe_sort_workspace",
+    "nvfp4_moe_sort",
+    "nvfp4_moe_gather",
+    "nvfp4_moe_gather_backward",
+    "nvfp4_moe_combine",
+    "nvfp4_moe_combine_backward",
 )
 
 _P = ctypes.c_void_p
@@ -51,6 +59,22 @@ class GemmArgs(ctypes.Structure):
                 ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("L", ctypes.c_int32),
                 ("a_lstride", _L), ("b_lstride", _L), ("sfa_lstride", _L), ("sfb_lstride", _L), ("ldc", _L),
                 ("c_lstride", _L), ("stream", _P)]
+
+
+class MxQuantArgs(ctypes.Structure):
+    """nvfp4_mx_quant_args of include/nvfp4_b200.h."""
+    _fields_ = [("x", _P), ("packed", _P), ("scales", _P), ("offsets", _P), ("slots", _P),
+                ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("K", ctypes.c_int32),
+                ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("columns", ctypes.c_int32),
+                ("x_rstride", _L), ("x_estride", _L), ("stream", _P)]
+
+
+class MoeArgs(ctypes.Structure):
+    """nvfp4_moe_args of include/nvfp4_b200.h."""
+    _fields_ = [("in_", _P), ("grad", _P), ("weights", _P), ("out", _P), ("dweights", _P), ("slots", _P),
+                ("offsets", _P), ("dtype", ctypes.c_int32), ("tokens", ctypes.c_int32), ("top", ctypes.c_int32),
+                ("hidden", ctypes.c_int32), ("experts", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("in_stride", _L), ("grad_stride", _L), ("stream", _P)]
 
 
 class Nvfp4Error(RuntimeError):
@@ -89,6 +113,16 @@ def load() -> ctypes.CDLL:
     for name in ("nvfp4_gemm_call", "nvfp4_dual_gemm_call"):
         getattr(lib, name).restype = _I
         getattr(lib, name).argtypes = [ctypes.POINTER(GemmArgs)]
+    for name in ("nvfp4_mx_quantize", "nvfp4_mx_dequantize"):
+        getattr(lib, name).restype = _I
+        getattr(lib, name).argtypes = [ctypes.POINTER(MxQuantArgs)]
+    lib.nvfp4_moe_sort_workspace.restype = _L
+    lib.nvfp4_moe_sort_workspace.argtypes = [_I, _I]
+    lib.nvfp4_moe_sort.restype = _I
+    lib.nvfp4_moe_sort.argtypes = [_P, _I, _I, _I, _P, _P, _P, _P, _L, _P]
+    for name in ("nvfp4_moe_gather", "nvfp4_moe_gather_backward", "nvfp4_moe_combine", "nvfp4_moe_combine_backward"):
+        getattr(lib, name).restype = _I
+        getattr(lib, name).argtypes = [ctypes.POINTER(MoeArgs)]
     _lib = lib
     return lib
 

@@ -235,6 +235,31 @@ typedef struct {
 int nvfp4_mx_quantize(const nvfp4_mx_quant_args* args);
 int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* args);
 
+/* Products of MXFP4 operands, fp32 sums, out_dtype 0 (fp16), 1 (bf16), 2 (fp32):
+ *   c[r, n] = sum_k a[r, k] b[e(r)][n, k],   or, with b2 and its scales,
+ *   c[r, n] = silu(a[r] . b[e(r)][n]) * (a[r] . b2[e(r)][n])
+ *   a       : codes [rows][K/2], scales as above
+ *   b, b2   : codes [experts][N][K/2], scales [experts][ceil(N/128)] row blocks
+ *   c       : [rows][ldc]
+ *   offsets : the rows are sorted by expert; NULL with experts == 1
+ * Any rows >= 0 and N >= 1, K % 32 == 0.  Needs no workspace: calls on several
+ * streams may overlap. */
+typedef struct {
+  const void* a;
+  const void* b;
+  const void* b2;
+  const void* sfa;
+  const void* sfb;
+  const void* sfb2;
+  void* c;
+  const int32_t* offsets;
+  int32_t rows, N, K, experts, out_dtype, reserved;
+  int64_t ldc;
+  void* stream;
+} nvfp4_mx_gemm_args;
+
+int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* args);
+
 /* Sorts n slots by expert, stably: ids[n] (int32 or int64: id_bytes 4, 8);
  * an id outside 0 .. experts-1 is not routed.
  *   order[n]           the slot of each sorted row, -1 behind the last

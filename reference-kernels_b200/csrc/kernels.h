@@ -158,6 +158,18 @@ struct MxQuantArgs {
 cudaError_t launch_mx_quantize(const MxQuantArgs& a, int num_sms, cudaStream_t stream);
 cudaError_t launch_mx_dequantize(const MxQuantArgs& a, int num_sms, cudaStream_t stream);
 
+// Products of MXFP4 operands (mx_gemm.cu).
+struct MxGemmArgs {
+  const void *a, *b, *b2, *sfa, *sfb, *sfb2;  // b2 null: not gated
+  void* c;
+  const int* offsets;  // rows sorted by expert (or null: one weight matrix)
+  int rows, N, K, experts, out_dtype;
+  int64_t ldc;
+  int* status;
+  int inject;
+};
+cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why);
+
 // Tokens sorted by expert and back (moe.cu).
 struct MoeSortArgs {
   const void* ids;  // [slots_n], int32 or int64 (id_bytes)

@@ -1,0 +1,693 @@
+// Products of MXFP4 operands (e2m1, one e8m0 scale per 32) for any number of
+// tokens, of one weight matrix or of one per expert:
+//
+//   y[r, n] = sum_k (a sa)[r, k] (b[e(r)] sb[e(r)])[n, k]               r: rows sorted by expert
+//   gated:    silu(a . b1^T) * (a . b2^T)
+//
+// fp32 sums in the tensor cores, rounded once to the output's type.
+//
+// The weights' rows take the M side of the tcgen05 tile and the tokens the N
+// side: M is 128 whatever the problem, while N goes down to the tokens that are
+// there (in steps of 32), so a decoding step pays for its few tokens and a
+// weight is never padded by more than a tile at the end of N.  Tiles of up to
+// `tn` tokens are cut within each expert's rows; a TMA box that reaches past an
+// expert's last row reads the next one's, whose products are not stored.
+// A gated tile is 64 rows of b1 over 64 rows of b2, so that both products of
+// an output share a tile, its token operand and its accumulator.
+//
+// One persistent CTA per SM, 13 warps:
+//   0, 10..12  TMA producers (K tiles of 256 dealt round-robin)
+//   1          TMEM owner, MMA issuer: tcgen05.mma kind::mxf4 block32, K = 64
+//   2..5       epilogue
+//   6..9       scale writers: each tile's 128x4 scale blocks from shared memory
+//              to TMEM (tcgen05.st; tcgen05.cp would take tensor-pipe time).  A
+//              token tile that begins inside a block of 128 takes its words from
+//              the block's middle on.
+// The offsets are read on the device: every CTA builds the table of the experts'
+// rows, scale blocks and tiles in shared memory and walks the same tile list, so
+// the host never waits for a routing.
+//
+// Few tiles (a decoding step of one matrix): a cluster splits K and adds its
+// partial sums through distributed shared memory, in rank order.
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "experts.cuh"
+#include "kernels.h"
+
+namespace nvfp4 {
+
+bool make_tma_3d_u8(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t L, uint64_t row_stride,
+                    uint64_t lstride, uint32_t box_inner, uint32_t box_rows);
+
+namespace {
+
+constexpr int kBM = 128;                 // weight rows per tile
+constexpr int kBK = 256;                 // K elements per stage: 128 bytes per row
+constexpr int kBKBytes = kBK / 2;
+constexpr int kABytes = kBM * kBKBytes;  // weight bytes per stage
+constexpr int kSfBytes = 1024;           // scales of 128 rows of one stage: two 512-byte blocks
+constexpr int kMaxProducers = 4;
+constexpr int kThreads = 416;
+constexpr int kMaxStages = 10;
+constexpr int kTmemCols = 512;
+constexpr int kChunk = 32;               // tokens per epilogue step
+constexpr int kSmemMax = 227 * 1024 - 128;  // dynamic; the rest is for the static abort flag
+
+struct Params {
+  const uint8_t* sfw;   // scales of the weights (b, b1)
+  const uint8_t* sfw2;  // of b2 (gated)
+  const uint8_t* sfx;   // scales of the tokens
+  void* c;
+  const int* offsets;  // null: one expert with all rows
+  int rows, N, K, experts;
+  int64_t ldc;
+  int tn;         // tokens per tile: 32, 64, 128, 192 or 256
+  int box;        // token rows per TMA box
+  int nblk;       // 128-row scale blocks that a token tile can touch
+  int stages, producers, acc_bufs;
+  int sf_cols;    // TMEM columns of scales per stage
+  int n_tiles;    // tiles along N
+  int splits;     // CTAs of a cluster that share a tile's K (kSplit)
+  int vec;        // 16-byte stores of C
+  int* status;
+  int inject;     // test hook: CTA 0 withholds its first weight load
+};
+
+// D (+)= (A x sfA) (B x sfB)^T, e2m1 operands, e8m0 scales, one per 32.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+
+// Instruction descriptor for kind::mxf4: e2m1 operands, e8m0 scales (bit 23);
+// of the four scale bytes in a TMEM word an MMA of K = 64 takes two, from byte
+// 0 or 2 (scale ids, bits 4-5 for B and 29-30 for A).
+__device__ __forceinline__ uint32_t idesc_mxf4(int n, uint32_t scale_id) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (8u << 24) | (scale_id << 4) |
+         (scale_id << 29);
+}
+
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+
+__device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool epi_all(bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.and.pred p, 1, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(out)
+      : "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return out != 0;
+}
+__device__ __forceinline__ void set_status(int* status, int code) {
+  if (status) atomicCAS(status, 0, code);
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_peer(uint32_t saddr, uint32_t rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(saddr), "r"(rank));
+  return out;
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3])
+               : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ float round_to<float>(float v) {
+  return v;
+}
+
+__device__ __forceinline__ float silu_mul(float x, float y) { return __fdividef(x, 1.0f + __expf(-x)) * y; }
+
+// The experts' rows, scale blocks and tiles, in shared memory: E + 1 ints each.
+struct Table {
+  const int *row, *blk, *tile;
+};
+
+struct Tile {
+  int e;       // expert
+  int row0;    // first row
+  int rows;    // rows of the tile, 1 .. tn
+  int in_blk;  // row0's place in its scale block, a multiple of 32
+  int blk;     // its scale block
+  int ft;      // tile along N
+};
+
+// Tile t (< tab.tile[E]); `e` is the walker's cursor.  Tiles of an expert go
+// over up to kGroup token tiles for each weight tile, so that CTAs that run
+// together share both operands in L2.
+constexpr int kGroup = 12;
+__device__ __forceinline__ Tile tile_at(const Params& p, const Table& tab, int t, int& e) {
+  while (t >= tab.tile[e + 1]) ++e;
+  const int count = tab.row[e + 1] - tab.row[e];
+  const int mt = (count + p.tn - 1) / p.tn;
+  int r = t - tab.tile[e];
+  const int g = r / (kGroup * p.n_tiles);
+  const int gm = min(mt - g * kGroup, kGroup);
+  r -= g * kGroup * p.n_tiles;
+  Tile o;
+  o.e = e;
+  o.ft = r / gm;
+  const int m0 = (g * kGroup + r - o.ft * gm) * p.tn;
+  o.row0 = tab.row[e] + m0;
+  o.rows = min(p.tn, count - m0);
+  o.in_blk = m0 & 127;
+  o.blk = tab.blk[e] + (m0 >> 7);
+  return o;
+}
+
+template <typename OutT, bool kGate, bool kSplit>
+__global__ void __launch_bounds__(kThreads, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
+                   const __grid_constant__ CUtensorMap tm_x, const Params p) {
+  constexpr int kF = kGate ? 64 : 128;  // output features per tile
+  constexpr int kSfW = kGate ? 2 : 1;   // weight scale blocks per 128 columns of K
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int S = p.stages;
+  const int stage_bytes = kABytes + p.tn * kBKBytes;
+  const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
+  uint8_t* sfbuf = smem + S * stage_bytes;
+  OutT* staging = reinterpret_cast<OutT*>(sfbuf + S * sf_bytes);  // two of kChunk x kF
+  float* exch = reinterpret_cast<float*>(staging + 2 * kChunk * kF);  // gated: kChunk x 64
+  uint64_t* bars = reinterpret_cast<uint64_t*>(exch + (kGate ? kChunk * 64 : 0));
+  uint64_t* full = bars;
+  uint64_t* empty = full + S;
+  uint64_t* sf_full = empty + S;
+  uint64_t* acc_full = sf_full + S;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* row_tab = reinterpret_cast<int*>(tmem_slot + 2);
+  int* blk_tab = row_tab + p.experts + 1;
+  int* tile_tab = blk_tab + p.experts + 1;
+  __shared__ volatile int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int KT = (p.K + kBK - 1) / kBK, K128 = (p.K + 127) >> 7;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1 + 4);  // the producer, and each scale writer
+      mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 128);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    prefetch_tensormap(&tm_w);
+    prefetch_tensormap(&tm_x);
+    if (kGate) prefetch_tensormap(&tm_w2);
+    pdl_allow_dependents();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
+  pdl_wait();
+  if (warp == 0) {
+    // Table of the experts, then the running number of their tiles.
+    if (p.offsets) {
+      load_expert_table(p.offsets, p.experts, p.rows, row_tab, blk_tab);
+    } else if (lane == 0) {
+      row_tab[0] = blk_tab[0] = 0;
+      row_tab[1] = p.rows;
+    }
+    __syncwarp();
+    int carry = 0;
+    for (int base = 0; base < p.experts; base += 32) {
+      const int e = base + lane;
+      int n = e < p.experts ? (row_tab[e + 1] - row_tab[e] + p.tn - 1) / p.tn * p.n_tiles : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, n, d);
+        if (lane >= d) n += o;
+      }
+      n += carry;
+      if (e < p.experts) tile_tab[e + 1] = n;
+      carry = __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) tile_tab[0] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t sf_col0 = p.acc_bufs * p.tn;
+  const Table tab{row_tab, blk_tab, tile_tab};
+  const int total = tile_tab[p.experts];
+  // Work of this CTA: tiles t0, t0 + step, .., K tiles [k0, k1) of each.
+  const int t0 = kSplit ? blockIdx.x / p.splits : blockIdx.x;
+  const int step = kSplit ? total : gridDim.x;  // kSplit: one tile per cluster
+  const int rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int k0 = kSplit ? rank * KT / p.splits : 0, k1 = kSplit ? (rank + 1) * KT / p.splits : KT;
+  bool partial_ready = false;  // epilogue threads, kSplit: this CTA's partial sums are in TMEM
+
+  const int producer = warp == 0 ? 0 : warp >= 10 ? warp - 9 : -1;
+  if (producer >= 0) {
+    // ------------------------------------------------------------ producers
+    if (lane == 0 && producer < p.producers) {
+      const uint64_t keep = policy_evict_last(), once = policy_evict_first();
+      int g = 0, e = 0;
+      const int wblocks = (p.N + 127) >> 7;
+      for (int t = t0; t < total && !abort_flag; t += step) {
+        const Tile o = tile_at(p, tab, t, e);
+        const int f0 = o.ft * kF;
+        const int64_t wsf = (static_cast<int64_t>(o.e) * wblocks + (f0 >> 7)) * K128 * 512;
+        const uint8_t* xsf = p.sfx + static_cast<int64_t>(o.blk) * K128 * 512;
+        const int nb = ((o.in_blk + o.rows - 1) >> 7) + 1;
+        const int boxes = (o.rows + p.box - 1) / p.box;
+        for (int kt = k0; kt < k1; ++kt, ++g) {
+          if (g % p.producers != producer) continue;
+          const int stage = g % S;
+          if (!mbar_wait(&empty[stage], ((g / S) & 1) ^ 1)) {
+            set_status(p.status, kStatusTimeoutEmpty);
+            abort_flag = 1;
+            break;
+          }
+          uint8_t* st = smem + stage * stage_bytes;
+          uint8_t* sf = sfbuf + stage * sf_bytes;
+          const uint32_t bytes = min(2, K128 - 2 * kt) * 512;
+          mbar_arrive_expect_tx(&sf_full[stage], (kSfW + nb) * bytes);
+          bulk_load(sf, p.sfw + wsf + kt * kSfBytes, bytes, &sf_full[stage], once);
+          if (kGate) bulk_load(sf + kSfBytes, p.sfw2 + wsf + kt * kSfBytes, bytes, &sf_full[stage], once);
+          for (int b = 0; b < nb; ++b)
+            bulk_load(sf + (kSfW + b) * kSfBytes, xsf + (static_cast<int64_t>(b) * K128 + 2 * kt) * 512, bytes,
+                      &sf_full[stage], keep);
+          mbar_arrive_expect_tx(&full[stage], kABytes + boxes * p.box * kBKBytes);
+          if (!(p.inject && blockIdx.x == 0 && t == t0 && kt == k0)) {
+            tma_load_3d(st, &tm_w, &full[stage], kt * kBKBytes, f0, o.e, once);
+            if (kGate) tma_load_3d(st + kABytes / 2, &tm_w2, &full[stage], kt * kBKBytes, f0, o.e, once);
+          }
+          for (int b = 0; b < boxes; ++b)
+            tma_load_3d(st + kABytes + b * p.box * kBKBytes, &tm_x, &full[stage], kt * kBKBytes, o.row0 + b * p.box, 0,
+                        keep);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      int stage = 0, acc = 0, e = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = t0; t < total && ok && !abort_flag; t += step) {
+        const Tile o = tile_at(p, tab, t, e);
+        const int n = (o.rows + 31) & ~31;
+        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1)) {
+          set_status(p.status, kStatusTimeoutAccEmpty);
+          abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * p.tn;
+        for (int kt = k0; kt < k1; ++kt) {
+          if (!mbar_wait(&full[stage], phase)) {
+            set_status(p.status, kStatusTimeoutFull);
+            abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + stage * stage_bytes);
+          const uint32_t sfw = tmem_base + sf_col0 + stage * p.sf_cols, sfx = sfw + 8;
+          const int steps = min(4, (p.K - kt * kBK + 63) >> 6);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < steps)
+              mma_mxf4(d, desc_kmajor_sw128(st + kk * 32), desc_kmajor_sw128(st + kABytes + kk * 32),
+                       idesc_mxf4(n, (kk & 1) * 2), sfw + 4 * (kk >> 1), sfx + 4 * p.nblk * (kk >> 1),
+                       kt != k0 || kk != 0);
+          tc_commit(&empty[stage]);
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit(&acc_full[acc]);
+        if (++acc == p.acc_bufs) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      // Every tcgen05 operation has retired before TMEM is freed.
+      tc_commit(drain);
+      mbar_wait(drain, 0);
+    }
+  } else if (warp >= 6) {
+    // ------------------------------------------------------------ scale writers
+    // Warp 6 + i writes lane quarter (6 + i) % 4.  Per 128 columns of K: the
+    // weight block at columns 4 * kb, the token blocks at 8 + 4 * nblk * kb;
+    // column c of an operand holds the words of its rows 32 c .. 32 c + 31.
+    const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    int stage = 0, e = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = t0; t < total && ok; t += step) {
+      const Tile o = tile_at(p, tab, t, e);
+      const int nb = ((o.in_blk + o.rows - 1) >> 7) + 1;
+      const int shift = o.in_blk >> 5;
+      const int half = ((o.ft * kF) & 127) >> 5;  // gated: the tile's first word in its weight blocks
+      for (int kt = k0; kt < k1; ++kt) {
+        const bool got = mbar_wait(&sf_full[stage], phase);
+        if (!__all_sync(0xffffffffu, got && !abort_flag)) {
+          if (lane == 0 && !got) set_status(p.status, kStatusTimeoutFull);
+          abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint8_t* sf = sfbuf + stage * sf_bytes + lane * 16;
+        const uint32_t col = tmem_base + quarter + sf_col0 + stage * p.sf_cols;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const int left = (p.K >> 5) - 4 * (2 * kt + kb);  // scales per row from here on
+          if (left <= 0) break;
+          // Padding columns are not the caller's to fill: read as 2^-127.
+          const uint32_t mask = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
+          uint4 v;
+          if (kGate) {
+            const uint2 v1 = *reinterpret_cast<const uint2*>(sf + kb * 512 + half * 4);
+            const uint2 v2 = *reinterpret_cast<const uint2*>(sf + kSfBytes + kb * 512 + half * 4);
+            v = make_uint4(v1.x, v1.y, v2.x, v2.y);
+          } else {
+            v = *reinterpret_cast<const uint4*>(sf + kb * 512);
+          }
+          tmem_st_32x32b_x4(col + 4 * kb, make_uint4(v.x & mask, v.y & mask, v.z & mask, v.w & mask));
+          const uint8_t* xs = sf + kSfW * kSfBytes + kb * 512;
+          uint4 a = *reinterpret_cast<const uint4*>(xs);
+          uint4 b = nb > 1 ? *reinterpret_cast<const uint4*>(xs + kSfBytes) : make_uint4(0, 0, 0, 0);
+          a = make_uint4(a.x & mask, a.y & mask, a.z & mask, a.w & mask);
+          b = make_uint4(b.x & mask, b.y & mask, b.z & mask, b.w & mask);
+          if (shift == 1) {
+            a = make_uint4(a.y, a.z, a.w, b.x);
+            b = make_uint4(b.y, b.z, b.w, 0);
+          } else if (shift == 2) {
+            a = make_uint4(a.z, a.w, b.x, b.y);
+            b = make_uint4(b.z, b.w, 0, 0);
+          } else if (shift == 3) {
+            a = make_uint4(a.w, b.x, b.y, b.z);
+            b = make_uint4(b.w, 0, 0, 0);
+          }
+          tmem_st_32x32b_x4(col + 8 + 4 * p.nblk * kb, a);
+          if (p.nblk > 1) tmem_st_32x32b_x4(col + 8 + 4 * p.nblk * kb + 4, b);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  }
+
+  // ------------------------------------------------------------ epilogue
+  const bool epi = warp >= 2 && warp <= 5;
+  const int q = warp & 3;
+  const int rloc = q * 32 + lane;  // TMEM lane: the tile's weight row
+  const uint32_t tquarter = static_cast<uint32_t>(q * 32) << 16;
+  OutT* const c = static_cast<OutT*>(p.c);
+  // W tokens (columns) of this thread's weight row to rows row0 .. of C, features
+  // f0 ..; `valid` tokens are stored.  Through shared memory, where a token's
+  // features lie together: 2-byte stores of a warp's 32 features side by side,
+  // then 16 bytes per thread.
+  int buf = 0;
+  auto emit = [&](auto width, const uint32_t* r, int64_t row0, int f0, int valid) {
+    constexpr int W = decltype(width)::value;
+    OutT* out = staging + buf * kChunk * kF;
+    buf ^= 1;
+    if (kGate) {
+      // Lanes 0..63 hold x1, 64..127 x2 of the same outputs: each half gives the
+      // other one half of the tokens and computes the rest.
+      const bool first = rloc < 64;
+      const int f = rloc & 63;
+      float* const give = exch + (first ? W / 2 : 0) * 64 + f;
+      const float* const take = exch + (first ? 0 : W / 2) * 64 + f;
+      OutT* const dst = out + (first ? 0 : W / 2) * kF + f;
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) give[i * 64] = __uint_as_float(first ? r[W / 2 + i] : r[i]);
+      epi_bar();
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) {
+        const float own = __uint_as_float(first ? r[i] : r[W / 2 + i]), other = take[i * 64];
+        dst[i * kF] = round_to<OutT>(silu_mul(first ? own : other, first ? other : own));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[i * kF + rloc] = round_to<OutT>(__uint_as_float(r[i]));
+    }
+    epi_bar();
+    constexpr int kPer = 16 / sizeof(OutT), kVecs = kF / kPer;
+    const int tid = threadIdx.x - 64;
+    if (p.vec) {
+      for (int i = tid; i < W * kVecs; i += 128) {
+        const int tok = i / kVecs, f = (i % kVecs) * kPer;
+        if (tok >= valid || f0 + f >= p.N) continue;
+        OutT* dst = c + (row0 + tok) * p.ldc + f0 + f;
+        if (f0 + f + kPer <= p.N) {
+          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out + tok * kF + f);
+        } else {
+          for (int j = 0; f0 + f + j < p.N; ++j) dst[j] = out[tok * kF + f + j];
+        }
+      }
+    } else {
+      for (int i = tid; i < W * kF; i += 128) {
+        const int tok = i / kF, f = i % kF;
+        if (tok < valid && f0 + f < p.N) c[(row0 + tok) * p.ldc + f0 + f] = out[i];
+      }
+    }
+  };
+  if (epi) {
+    int acc = 0, e = 0;
+    uint32_t acc_phase = 0;
+    for (int t = t0; t < total; t += step) {
+      const Tile o = tile_at(p, tab, t, e);
+      // The four warps agree before any goes on to the named barriers.
+      if (!epi_all(mbar_wait(&acc_full[acc], acc_phase))) {
+        if (threadIdx.x == 64) set_status(p.status, kStatusTimeoutAccFull);
+        abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      if (kSplit) {
+        partial_ready = true;
+        break;
+      }
+      const uint32_t tacc = tmem_base + tquarter + acc * p.tn;
+      for (int c0 = 0; c0 < o.rows; c0 += kChunk) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tacc + c0, r);
+        tmem_wait_ld();
+        if (c0 + kChunk >= o.rows) {
+          tc_fence_before();
+          mbar_arrive(&acc_empty[acc]);
+        }
+        emit(std::integral_constant<int, 32>(), r, o.row0 + c0, o.ft * kF, min(kChunk, o.rows - c0));
+      }
+      if (++acc == p.acc_bufs) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    // Rows that belong to no expert.
+    const int tid = threadIdx.x - 64;
+    for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
+      for (int f = tid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
+  }
+
+  if (kSplit && t0 < total) {
+    // ---------------------------------------------------------- partial sums of a cluster
+    // Groups of 8 tokens are dealt to the ranks in contiguous shares; each rank
+    // sends its partial sums of the other ranks' shares to their shared memory
+    // (the pipeline's, free once every rank is past its main loop) and adds up
+    // its own share, own sums first and then by rank: the same order always.
+    const bool ok = epi ? epi_all(partial_ready) : true;
+    tc_fence_after();
+    cluster_sync_all();
+    int e = 0;
+    const Tile o = tile_at(p, tab, t0, e);
+    const int ng = (o.rows + 7) >> 3;
+    const int share = (ng + p.splits - 1) / p.splits;
+    const uint32_t tacc = tmem_base + tquarter;
+    auto at = [&](int slot, int gi, int half) {
+      return static_cast<uint32_t>((((slot * share + gi) * 2 + half) * kBM + rloc) * 16);
+    };
+    if (epi && ok) {
+      for (int i = 1; i < p.splits; ++i) {
+        const int peer = (rank + i) % p.splits;
+        const uint32_t base = map_peer(smem_u32(smem), peer);
+        const int slot = rank < peer ? rank : rank - 1;
+        for (int g = peer * share; g < min(ng, (peer + 1) * share); ++g) {
+          uint32_t r[8];
+          tmem_ld_32x32b_x8(tacc + 8 * g, r);
+          tmem_wait_ld();
+          st_cluster_v4(base + at(slot, g - peer * share, 0), r);
+          st_cluster_v4(base + at(slot, g - peer * share, 1), r + 4);
+        }
+      }
+    }
+    cluster_sync_all();
+    if (epi && ok) {
+      for (int g = rank * share; g < min(ng, (rank + 1) * share); ++g) {
+        uint32_t r[8];
+        tmem_ld_32x32b_x8(tacc + 8 * g, r);
+        tmem_wait_ld();
+        for (int slot = 0; slot < p.splits - 1; ++slot)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 v = *reinterpret_cast<const float4*>(smem + at(slot, g - rank * share, h));
+            r[4 * h] = __float_as_uint(__uint_as_float(r[4 * h]) + v.x);
+            r[4 * h + 1] = __float_as_uint(__uint_as_float(r[4 * h + 1]) + v.y);
+            r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
+            r[4 * h + 3] = __float_as_uint(__uint_as_float(r[4 * h + 3]) + v.w);
+          }
+        emit(std::integral_constant<int, 8>(), r, o.row0 + 8 * g, o.ft * kF, min(8, o.rows - 8 * g));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+size_t fixed_smem(int out_size, bool gate, int experts) {
+  const int f = gate ? 64 : 128;
+  return 1024 /* alignment */ + 2 * kChunk * f * out_size + (gate ? kChunk * 64 * 4 : 0) +
+         (3 * kMaxStages + 6) * 8 + 8 + 3 * (static_cast<size_t>(experts) + 1) * 4;
+}
+
+template <typename OutT, bool kGate, bool kSplit>
+cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream, const char** why) {
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  auto kernel = mx_gemm_kernel<OutT, kGate, kSplit>;
+  if (dev >= 64 || !attr_done[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_done[dev] = true;
+  }
+  CUtensorMap tw, tw2, tx;
+  const uint64_t k2 = g.K / 2, n = g.N;
+  const uint32_t wbox = kGate ? 64 : 128;
+  if (!make_tma_3d_u8(&tw, g.b, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox) ||
+      (kGate && !make_tma_3d_u8(&tw2, g.b2, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox)) ||
+      !make_tma_3d_u8(&tx, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, p.box)) {
+    *why = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kSplit ? p.splits : 1, tw, kGate ? tw2 : tw, tx,
+                    p);
+}
+
+template <typename OutT>
+cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream,
+                       const char** why) {
+  if (p.splits > 1)
+    return g.b2 ? launch<OutT, true, true>(g, p, smem, grid, stream, why)
+                : launch<OutT, false, true>(g, p, smem, grid, stream, why);
+  return g.b2 ? launch<OutT, true, false>(g, p, smem, grid, stream, why)
+              : launch<OutT, false, false>(g, p, smem, grid, stream, why);
+}
+
+}  // namespace
+
+cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why) {
+  const bool gate = g.b2 != nullptr;
+  const int out_size = g.out_dtype == 2 ? 4 : 2;
+  Params p{};
+  p.sfw = static_cast<const uint8_t*>(g.sfb);
+  p.sfw2 = static_cast<const uint8_t*>(g.sfb2);
+  p.sfx = static_cast<const uint8_t*>(g.sfa);
+  p.c = g.c;
+  p.offsets = g.offsets;
+  p.rows = g.rows;
+  p.N = g.N;
+  p.K = g.K;
+  p.experts = g.experts;
+  p.ldc = g.ldc;
+  p.status = g.status;
+  p.inject = g.inject;
+  p.vec = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
+  p.n_tiles = (g.N + (gate ? 63 : 127)) / (gate ? 64 : 128);
+  // Tokens per tile: the smallest that holds an average expert's rows with
+  // room for an uneven routing (an expert over the tile reads its weights twice).
+  const int busy = g.experts < g.rows ? g.experts : g.rows;
+  const int avg = (g.rows + busy - 1) / busy;
+  const int want = g.offsets ? avg + avg / 2 : avg;
+  p.tn = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 192;
+  p.box = p.tn < 64 ? p.tn : 64;
+  p.nblk = p.tn <= 128 ? 1 : 2;
+  p.acc_bufs = p.tn <= 192 ? 2 : 1;
+  p.sf_cols = 8 + 8 * p.nblk;
+  // Stages: what shared memory and TMEM hold.
+  const size_t fixed = fixed_smem(out_size, gate, g.experts);
+  const size_t stage = kABytes + p.tn * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;
+  int stages = static_cast<int>((kSmemMax - fixed) / stage);
+  const int tmem_stages = (kTmemCols - p.acc_bufs * p.tn) / p.sf_cols;
+  stages = stages < tmem_stages ? stages : tmem_stages;
+  p.stages = stages < kMaxStages ? stages : kMaxStages;
+  // A producer waits on a stage by phase parity, which is exact only while it
+  // waits for every stage at most one lap behind: not more producers than stages.
+  p.producers = p.stages < kMaxProducers ? p.stages : kMaxProducers;
+  // Tiles at most (whatever the offsets), and K splits where they leave SMs idle.
+  const int64_t tiles = (static_cast<int64_t>(g.rows) / p.tn + busy) * p.n_tiles;
+  const int64_t exact = g.offsets ? tiles : static_cast<int64_t>((g.rows + p.tn - 1) / p.tn) * p.n_tiles;
+  const int KT = (g.K + kBK - 1) / kBK;
+  p.splits = 1;
+  if (p.tn <= 128)
+    while (p.splits < 8 && exact * p.splits * 2 <= num_sms && KT >= p.splits * 4) p.splits *= 2;
+  const int64_t grid = p.splits > 1 ? exact * p.splits : exact < num_sms ? exact : num_sms;
+  const size_t smem = fixed + p.stages * stage;
+  return g.out_dtype == 0   ? launch_out<__half>(g, p, smem, static_cast<int>(grid), stream, why)
+         : g.out_dtype == 1 ? launch_out<__nv_bfloat16>(g, p, smem, static_cast<int>(grid), stream, why)
+                            : launch_out<float>(g, p, smem, static_cast<int>(grid), stream, why);
+}
+
+}  // namespace nvfp4

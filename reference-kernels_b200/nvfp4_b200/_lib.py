@@ -30,6 +30,7 @@ EXPORTS = (
     "nvfp4_dual_gemm_call",
     "nvfp4_mx_quantize",
     "nvfp4_mx_dequantize",
+    "nvfp4_mx_gemm",
     "nvfp4_moe_sort_workspace",
     "nvfp4_moe_sort",
     "nvfp4_moe_gather",
@@ -67,6 +68,13 @@ class MxQuantArgs(ctypes.Structure):
                 ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32), ("K", ctypes.c_int32),
                 ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("columns", ctypes.c_int32),
                 ("x_rstride", _L), ("x_estride", _L), ("stream", _P)]
+
+
+class MxGemmArgs(ctypes.Structure):
+    """nvfp4_mx_gemm_args of include/nvfp4_b200.h."""
+    _fields_ = [("a", _P), ("b", _P), ("b2", _P), ("sfa", _P), ("sfb", _P), ("sfb2", _P), ("c", _P), ("offsets", _P),
+                ("rows", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("experts", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("ldc", _L), ("stream", _P)]
 
 
 class MoeArgs(ctypes.Structure):
@@ -116,6 +124,8 @@ def load() -> ctypes.CDLL:
     for name in ("nvfp4_mx_quantize", "nvfp4_mx_dequantize"):
         getattr(lib, name).restype = _I
         getattr(lib, name).argtypes = [ctypes.POINTER(MxQuantArgs)]
+    lib.nvfp4_mx_gemm.restype = _I
+    lib.nvfp4_mx_gemm.argtypes = [ctypes.POINTER(MxGemmArgs)]
     lib.nvfp4_moe_sort_workspace.restype = _L
     lib.nvfp4_moe_sort_workspace.argtypes = [_I, _I]
     lib.nvfp4_moe_sort.restype = _I

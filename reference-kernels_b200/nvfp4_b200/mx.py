@@ -28,6 +28,7 @@ import torch
 
 from . import _lib
 from .inputs import FP4X2
+from .ops import _post
 
 E8M0 = torch.float8_e8m0fnu
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -147,3 +148,42 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor
                                 matrices if experts is None else experts, 0, 0, k, rows * k, _raw_stream(dev))
         _lib.check(_lib.load().nvfp4_mx_dequantize(_byref(args)))
     return out
+
+
+def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype):
+    _require(out_dtype in _DTYPES, f"{who}: out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
+    experts = None
+    if offsets is not None:
+        experts = _experts(who, offsets)
+        _require(b1.dim() == 3 and b1.shape[0] == experts,
+                 f"{who}: offsets of {experts} experts need weights [{experts}, N, K/2], got {tuple(b1.shape)}")
+    _, rows, k = _check_operand(who, a, sa, 2, experts)
+    for b, s in ((b1, s1), (b2, s2)):
+        if b is not None:
+            _, n, kb = _check_operand(who, b, s, 2 if experts is None else 3)
+            _require(kb == k and b.shape == b1.shape, f"{who}: weights {tuple(b.shape)} do not fit tokens with K={k}"
+                     + ("" if b is b1 else f" and weights {tuple(b1.shape)}"))
+    dev = _device(who, a, sa, b1, s1, b2, s2, offsets)
+    c = torch.empty((rows, n), dtype=out_dtype, device=a.device)
+    if c.numel():
+        args = _lib.MxGemmArgs(a.data_ptr(), b1.data_ptr(), None if b2 is None else b2.data_ptr(), sa.data_ptr(),
+                               s1.data_ptr(), None if b2 is None else s2.data_ptr(), c.data_ptr(),
+                               None if offsets is None else offsets.data_ptr(), rows, n, k, experts or 1,
+                               _DTYPES[out_dtype], 0, n, _raw_stream(dev))
+        _lib.check(_lib.load().nvfp4_mx_gemm(_byref(args)))
+        _post()
+    return c
+
+
+def gemm(a, sa, b, sb, offsets: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [rows, K] times the transpose of b [N, K] -> [rows, N], for any number of rows.
+
+    With offsets, the rows are sorted by expert, b is [experts, N, K] and each row meets its expert's matrix; rows
+    behind the last expert's come out as zeros."""
+    return _product("mx.gemm", a, sa, b, sb, None, None, offsets, out_dtype)
+
+
+def dual_gemm(a, sa, b1, sb1, b2, sb2, offsets: torch.Tensor | None = None,
+              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """silu(a . b1^T) * (a . b2^T), otherwise as gemm; both products stay in fp32."""
+    return _product("mx.dual_gemm", a, sa, b1, sb1, b2, sb2, offsets, out_dtype)

@@ -1,0 +1,294 @@
+"""Products of MXFP4 operands.  With scales of a few binades every partial sum
+is a multiple of 2^-2 times a power of two and below 2^24 of them, so fp32 holds
+it whatever the order of the additions: the products must then be the 64-bit
+result rounded once, exactly."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from nvfp4_b200 import _lib, mx
+from tests import mxref
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def f64(t):
+    return t.double().cpu().numpy()
+
+
+def operand(rows, k, g, low=126, high=129, fill=255):
+    """codes, scale bytes; padding of the stored scales is 255 (NaN) to show that nobody reads it."""
+    return g.randint(0, 16, (rows, k)).astype(np.uint8), g.randint(low, high, (rows, k // 32)).astype(np.uint8)
+
+
+def on_gpu(codes, scales, at=None, blocks=None):
+    return (torch.from_numpy(mxref.pack(codes)).cuda(),
+            torch.from_numpy(mxref.blocked_scales(scales, at, blocks, fill=255)).cuda())
+
+
+def weights_on_gpu(ops):
+    parts = [on_gpu(*o) for o in ops]
+    return torch.stack([p[0] for p in parts]), torch.stack([p[1] for p in parts])
+
+
+def same(got, want):
+    np.testing.assert_array_equal(f64(got), f64(torch.from_numpy(want).to(got.dtype)))
+
+
+def gated(x1, x2):
+    with np.errstate(over="ignore"):
+        return x1 / (1 + np.exp(-x1)) * x2
+
+
+def gate_close(got, x1, x2):
+    """Half a step of the type, and of fp32: expf's 2 + 1.2 |x| units (its argument is scaled by log2 e in fp32), 2 of
+    the quotient, 1 of the sum, half of the product, each of 2^-23."""
+    want = gated(x1, x2)
+    eps = torch.finfo(got.dtype).eps
+    bound = np.abs(want) * (eps / 2 + (6 + 1.2 * np.abs(x1)) * 2.0 ** -23) + 1e-35 * np.abs(x2)
+    bound = bound + float(torch.finfo(got.dtype).smallest_normal) * eps / 2
+    d = np.abs(f64(got) - want)
+    assert (d <= bound).all(), (d / np.maximum(bound, 1e-300)).max()
+
+
+# ---------------------------------------------------------------- CPU
+def test_refusals():
+    a, sa = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((1, 1, 32, 4, 4), dtype=torch.uint8)
+    b, sb = torch.zeros((8, 32), dtype=torch.uint8), torch.zeros((1, 1, 32, 4, 4), dtype=torch.uint8)
+    with pytest.raises(_lib.Nvfp4Error, match="CUDA"):
+        mx.gemm(a, sa, b, sb)
+    off = torch.zeros(3, dtype=torch.int32)
+    for call, what in [
+            (lambda: mx.gemm(a, sa, b, sb, out_dtype=torch.float64), "out_dtype"),
+            (lambda: mx.gemm(a[:, :16].contiguous(), sa, torch.zeros((8, 48), dtype=torch.uint8), sb), "do not fit"),
+            (lambda: mx.gemm(a, sa, b, sa[:0]), "scales"),
+            (lambda: mx.gemm(a.float(), sa, b, sb), "codes"),
+            (lambda: mx.gemm(a[:, ::2], sa, b, sb), "codes"),
+            (lambda: mx.gemm(a, sa, b, sb, offsets=off), "2 experts"),
+            (lambda: mx.gemm(a, sa, b.view(1, 8, 32), sb.view(1, 1, 1, 32, 4, 4)), "2 dimensions"),
+            (lambda: mx.dual_gemm(a, sa, b, sb, b[:4], sb), "do not fit"),
+            (lambda: mx.gemm(a, sa, b.view(2, 4, 32), sb.expand(2, 1, 1, 32, 4, 4).contiguous(), offsets=off),
+             "scales")]:
+        with pytest.raises(_lib.Nvfp4Error, match=what):
+            call()
+
+
+def test_c_refusals():
+    lib, fake = _lib.load(), 1 << 20
+    d = dict(a=fake, b=fake, sfa=fake, sfb=fake, c=fake, rows=4, N=8, K=64, experts=1, out_dtype=1, ldc=8)
+
+    def rc(**kw):
+        return lib.nvfp4_mx_gemm(ctypes.byref(_lib.MxGemmArgs(**{**d, **kw})))
+
+    assert lib.nvfp4_mx_gemm(None) == 3
+    assert rc(out_dtype=3) == 1 and rc(rows=-1) == 1 and rc(N=0) == 1 and rc(K=48) == 1 and rc(K=0) == 1
+    assert rc(experts=0) == 1 and rc(experts=1025, offsets=fake) == 1 and rc(ldc=7) == 1
+    assert rc(rows=2 ** 31 - 1, N=2 ** 31 - 1, ldc=2 ** 31) == 1 and rc(K=1 << 25) == 1
+    assert rc(experts=2) == 3 and rc(a=None) == 3 and rc(b2=fake) == 3 and rc(sfb2=fake) == 3
+    assert rc(a=fake + 8) == 2 and rc(sfb=fake + 8) == 2 and rc(c=fake + 1) == 2 and rc(offsets=fake + 2) == 2
+
+
+def test_struct_layout_matches_header(tmp_path):
+    import os
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("gcc not available")
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "nvfp4_b200.h")
+    structs = {"nvfp4_mx_quant_args": _lib.MxQuantArgs, "nvfp4_mx_gemm_args": _lib.MxGemmArgs,
+               "nvfp4_moe_args": _lib.MoeArgs}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void) {"]
+    for name, py in structs.items():
+        lines.append(f'  printf("%zu\\n", sizeof({name}));')
+        lines += [f'  printf("%zu\\n", offsetof({name}, {f[0].rstrip("_")}));' for f in py._fields_]
+    (tmp_path / "l.c").write_text("\n".join(lines + ["  return 0;", "}"]))
+    subprocess.run(["gcc", str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "l")], capture_output=True, text=True).stdout.split()]
+    want = []
+    for py in structs.values():
+        want += [ctypes.sizeof(py)] + [getattr(py, f[0]).offset for f in py._fields_]
+    assert got == want
+
+
+# ---------------------------------------------------------------- GPU: one matrix
+SIZES = [(1, 1, 32), (1, 128, 256), (5, 7, 64), (31, 130, 96), (33, 64, 160), (64, 257, 1024), (100, 300, 544),
+         (130, 128, 7168), (193, 200, 288), (256, 129, 512), (385, 640, 320), (1000, 384, 736), (2049, 72, 128),
+         # few tiles and a long K: shared by the CTAs of a cluster
+         (1, 128, 8192), (17, 300, 4096), (70, 130, 4096), (128, 128, 16384), (2, 4096, 1024 + 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_gemm_is_exact(dtype, m, n, k):
+    g = np.random.RandomState(m + n + k)
+    a, b = operand(m, k, g), operand(n, k, g)
+    want = mxref.decode(*a) @ mxref.decode(*b).T
+    got = mx.gemm(*on_gpu(*a), *on_gpu(*b), out_dtype=dtype)
+    assert got.shape == (m, n) and got.dtype == dtype
+    same(got, want)
+    assert torch.equal(got, mx.gemm(*on_gpu(*a), *on_gpu(*b), out_dtype=dtype))
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [s for s in SIZES if s[2] <= 8192])
+def test_dual_gemm(dtype, m, n, k):
+    g = np.random.RandomState(m + n + k)
+    # a small enough that the gate's argument spans both sides of its bend
+    low = 127 - int(np.log2(k) / 2) - 4
+    a, b1, b2 = operand(m, k, g, low, low + 3), operand(n, k, g), operand(n, k, g)
+    x = mxref.decode(*a)
+    got = mx.dual_gemm(*on_gpu(*a), *on_gpu(*b1), *on_gpu(*b2), out_dtype=dtype)
+    gate_close(got, x @ mxref.decode(*b1).T, x @ mxref.decode(*b2).T)
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(3, 4096), (40, 1024), (200, 512)])
+def test_scales_over_their_range(m, k):
+    """Scales of all binades: |error| <= the fp32 error of a sum of k terms in any order, each addition off by up to a
+    whole step (the tensor core may cut instead of rounding)."""
+    g = np.random.RandomState(k)
+    a, b = operand(m, k, g, 60, 190), operand(96, k, g, 100, 150)
+    x, w = mxref.decode(*a), mxref.decode(*b)
+    want, magnitude = x @ w.T, np.abs(x) @ np.abs(w).T
+    got = f64(mx.gemm(*on_gpu(*a), *on_gpu(*b), out_dtype=torch.float32))
+    assert (np.abs(got - want) <= k * 2.0 ** -23 * magnitude).all()
+    # and in practice far less: the largest terms decide
+    assert np.median(np.abs(got - want) / magnitude) < 2.0 ** -22
+
+
+@pytest.mark.gpu
+def test_nan_blocks_reach_only_their_rows_and_columns():
+    g = np.random.RandomState(4)
+    m, n, k = 70, 150, 512
+    a, b = operand(m, k, g), operand(n, k, g)
+    a[1][13, 5] = 255
+    b[1][77, 15] = 255
+    got = f64(mx.gemm(*on_gpu(*a), *on_gpu(*b), out_dtype=torch.float32))
+    bad = np.zeros((m, n), bool)
+    bad[13], bad[:, 77] = True, True
+    assert np.isnan(got[bad]).all()
+    a[1][13, 5], b[1][77, 15] = 127, 127
+    want = mxref.decode(*a) @ mxref.decode(*b).T
+    np.testing.assert_array_equal(got[~bad], want[~bad])
+
+
+# ---------------------------------------------------------------- GPU: experts
+GROUPS = [([5], 0), ([0, 0, 0], 9), ([1, 0, 40, 0, 0, 3], 5), ([130, 1, 0, 127, 128, 129], 0), ([300, 0, 5], 20),
+          ([2] * 64, 3), ([1000, 3, 250], 1), ([0] * 500 + [7] + [0] * 523, 2), ([33] * 12, 0), ([70, 65, 64, 100], 0)]
+
+
+def grouped(counts, tail, n, k, seed, both=False):
+    g = np.random.RandomState(seed)
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    rows, used = sum(counts) + tail, sum(counts)
+    low = 127 - int(np.log2(k) / 2) - 4 if both else 126
+    a = operand(rows, k, g, low, low + 3)
+    at, _ = mxref.scale_rows(offsets)
+    ops = on_gpu(a[0], a[1][:used], at, min(rows, len(counts)) + rows // 128)
+    bs = [[operand(n, k, g) for _ in counts] for _ in range(2 if both else 1)]
+    x = mxref.decode(*a)
+    want = [np.concatenate([x[lo:hi] @ mxref.decode(*w).T for lo, hi, w in zip(offsets[:-1], offsets[1:], ws)]
+                           + [np.zeros((tail, n))]) for ws in bs]
+    return ops, [weights_on_gpu(ws) for ws in bs], torch.tensor(offsets, dtype=torch.int32).cuda(), want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(136, 288), (65, 512), (128, 1024)])
+@pytest.mark.parametrize("counts,tail", GROUPS)
+def test_experts(dtype, counts, tail, n, k):
+    if len(counts) > 100:
+        n, k = 33, 64
+    a, (b,), offsets, (want,) = grouped(counts, tail, n, k, 1)
+    same(mx.gemm(*a, *b, offsets=offsets, out_dtype=dtype), want)
+    a, (b1, b2), offsets, (x1, x2) = grouped(counts, tail, n, k, 2, both=True)
+    got = mx.dual_gemm(*a, *b1, *b2, offsets=offsets, out_dtype=dtype)
+    used = sum(counts)
+    gate_close(got[:used], x1[:used], x2[:used])
+    assert not f64(got[used:]).any()
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+def test_offsets_that_fall_or_leave_the_rows_stay_in_bounds():
+    g = np.random.RandomState(8)
+    rows, n, k, experts = 200, 72, 96, 3
+    bs = [operand(n, k, g) for _ in range(experts)]
+    weights = weights_on_gpu(bs)
+    for offsets in ([0, 500, 10, 200], [150, 150, 20, 0], [0, 60, 40, 1 << 30]):
+        clamped = np.maximum.accumulate(np.clip(offsets, 0, rows))
+        a = operand(rows, k, g)
+        at, _ = mxref.scale_rows(clamped)
+        lo, hi = clamped[0], clamped[-1]
+        ops = on_gpu(a[0], a[1][lo:hi], at, experts + rows // 128)
+        got = mx.gemm(*ops, *weights, offsets=torch.tensor(offsets, dtype=torch.int32).cuda())
+        want = np.concatenate([mxref.decode(a[0][s:t], a[1][s:t]) @ mxref.decode(*w).T
+                               for s, t, w in zip(clamped[:-1], clamped[1:], bs)])
+        same(got[lo:hi], want)
+        assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+def test_empty():
+    b = torch.zeros((8, 32), dtype=torch.uint8, device="cuda")
+    sb = torch.zeros((1, 1, 32, 4, 4), dtype=torch.uint8, device="cuda")
+    assert mx.gemm(b[:0], sb[:0], b, sb).shape == (0, 8)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert mx.gemm(b[:0], sb[:0], b.view(2, 4, 32), torch.stack([sb, sb]), offsets=off).shape == (0, 4)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_and_graphs():
+    """Products need no workspace: two streams, and two graphs, run side by side."""
+    g = np.random.RandomState(11)
+    cases = []
+    for m, n, k in ((3, 256, 4096), (500, 256, 512)):
+        a, b = operand(m, k, g), operand(n, k, g)
+        cases.append((on_gpu(*a) + on_gpu(*b), mxref.decode(*a) @ mxref.decode(*b).T))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = []
+    for _ in range(4):
+        for s, (ops, want) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                outs.append((mx.gemm(*ops), want))
+    torch.cuda.synchronize()
+    for got, want in outs:
+        same(got, want)
+    graphs = []
+    for ops, want in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = mx.gemm(*ops)
+        graphs.append((graph, out, want))
+    for graph, out, _ in graphs:
+        out.zero_()
+    torch.cuda.synchronize()
+    for s, (graph, out, want) in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    for graph, out, want in graphs:
+        same(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 128, 8192), (300, 256, 512)])
+def test_withheld_load_is_reported(monkeypatch, m, n, k):
+    """A load that never comes ends in a status within the waits' limit, and the next call is right again."""
+    g = np.random.RandomState(2)
+    a, b = operand(m, k, g), operand(n, k, g)
+    ops = on_gpu(*a) + on_gpu(*b)
+    monkeypatch.setenv("NVFP4_FAULT_INJECT", "1")
+    mx.gemm(*ops)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("NVFP4_FAULT_INJECT")
+    assert _lib.device_status(True) != 0
+    same(mx.gemm(*ops), mxref.decode(*a) @ mxref.decode(*b).T)
+    assert _lib.device_status(True) == 0

@@ -54,6 +54,7 @@ constexpr int kThreads = 416;
 constexpr int kMaxStages = 10;
 constexpr int kTmemCols = 512;
 constexpr int kChunk = 32;               // tokens per epilogue step
+constexpr int kSmallBox = 32;            // token rows of a small TMA box
 constexpr int kSmemMax = 227 * 1024 - 128;  // dynamic; the rest is for the static abort flag
 
 struct Params {
@@ -65,34 +66,47 @@ struct Params {
   int rows, N, K, experts;
   int64_t ldc;
   int tn;         // tokens per tile: 32, 64, 128, 192 or 256
-  int box;        // token rows per TMA box
   int nblk;       // 128-row scale blocks that a token tile can touch
   int stages, producers, acc_bufs;
   int sf_cols;    // TMEM columns of scales per stage
   int n_tiles;    // tiles along N
-  int splits;     // CTAs of a cluster that share a tile's K (kSplit)
+  int splits;     // CTAs of a cluster that share a tile's K (kSplitK)
+  int pair;       // kPairs
   int vec;        // 16-byte stores of C
   int* status;
   int inject;     // test hook: CTA 0 withholds its first weight load
 };
 
-// D (+)= (A x sfA) (B x sfB)^T, e2m1 operands, e8m0 scales, one per 32.
+// How CTAs share the tiles: one each; K split over a cluster; two CTAs a tile.
+enum Mode { kWhole, kSplitK, kPairs };
+
+// D (+)= (A x sfA) (B x sfB)^T, e2m1 operands, e8m0 scales, one per 32; kTwo:
+// of a pair of CTAs (M = 256, each CTA's rows of A and half of B's).
+template <bool kTwo>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-      : "memory");
+  if (kTwo)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+        : "memory");
 }
 
 // Instruction descriptor for kind::mxf4: e2m1 operands, e8m0 scales (bit 23);
 // of the four scale bytes in a TMEM word an MMA of K = 64 takes two, from byte
 // 0 or 2 (scale ids, bits 4-5 for B and 29-30 for A).
-__device__ __forceinline__ uint32_t idesc_mxf4(int n, uint32_t scale_id) {
-  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (8u << 24) | (scale_id << 4) |
-         (scale_id << 29);
+__device__ __forceinline__ uint32_t idesc_mxf4(int m, int n, uint32_t scale_id) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(m >> 4) << 24) | (scale_id << 4) | (scale_id << 29);
 }
 
 __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -102,36 +116,36 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                : "memory");
 }
 
-__device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool epi_all(bool pred) {
-  uint32_t out;
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[8], const uint32_t (&s)[8]) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.and.pred p, 1, 128, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(out)
-      : "r"(static_cast<uint32_t>(pred))
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(s[0]), "r"(s[1]),
+      "r"(s[2]), "r"(s[3]), "r"(s[4]), "r"(s[5]), "r"(s[6]), "r"(s[7])
       : "memory");
-  return out != 0;
 }
-__device__ __forceinline__ void set_status(int* status, int code) {
-  if (status) atomicCAS(status, 0, code);
+__device__ __forceinline__ void put4(uint32_t* dst, const uint8_t* src) {
+  const uint4 v = *reinterpret_cast<const uint4*>(src);
+  dst[0] = v.x;
+  dst[1] = v.y;
+  dst[2] = v.z;
+  dst[3] = v.w;
 }
-__device__ __forceinline__ void cluster_sync_all() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+// One lane of a converged warp, the same on every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t map_peer(uint32_t saddr, uint32_t rank) {
-  uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(saddr), "r"(rank));
-  return out;
-}
+
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3])
@@ -152,8 +166,6 @@ template <>
 __device__ __forceinline__ float round_to<float>(float v) {
   return v;
 }
-
-__device__ __forceinline__ float silu_mul(float x, float y) { return __fdividef(x, 1.0f + __expf(-x)) * y; }
 
 // The experts' rows, scale blocks and tiles, in shared memory: E + 1 ints each.
 struct Table {
@@ -192,16 +204,19 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Table& tab, int t
   return o;
 }
 
-template <typename OutT, bool kGate, bool kSplit>
+template <typename OutT, bool kGate, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-                   const __grid_constant__ CUtensorMap tm_x, const Params p) {
+                   const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_xs,
+                   const Params p) {
   constexpr int kF = kGate ? 64 : 128;  // output features per tile
   constexpr int kSfW = kGate ? 2 : 1;   // weight scale blocks per 128 columns of K
+  constexpr bool kSplit = kMode == kSplitK, kPair = kMode == kPairs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int S = p.stages;
-  const int stage_bytes = kABytes + p.tn * kBKBytes;
+  const int x_rows = kPair ? p.tn / 2 : p.tn;  // token rows of a stage
+  const int stage_bytes = kABytes + x_rows * kBKBytes;
   const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
   uint8_t* sfbuf = smem + S * stage_bytes;
   OutT* staging = reinterpret_cast<OutT*>(sfbuf + S * sf_bytes);  // two of kChunk x kF
@@ -219,28 +234,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* tile_tab = blk_tab + p.experts + 1;
   __shared__ volatile int abort_flag;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int KT = (p.K + kBK - 1) / kBK, K128 = (p.K + 127) >> 7;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1 + 4);  // the producer, and each scale writer
+      mbar_init(&full[s], kPair ? 1 + 8 : 1 + 4);  // the producer, and each scale writer (of both CTAs)
       mbar_init(&empty[s], 1);
       mbar_init(&sf_full[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 128);
+      mbar_init(&acc_empty[b], kPair ? 256 : 128);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
+    prefetch_tensormap(&tm_xs);
     if (kGate) prefetch_tensormap(&tm_w2);
     pdl_allow_dependents();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == 1) {
+    if (kPair)
+      tmem_alloc_pair(tmem_slot, kTmemCols);
+    else
+      tmem_alloc(tmem_slot, kTmemCols);
+  }
   pdl_wait();
   if (warp == 0) {
     // Table of the experts, then the running number of their tiles.
@@ -267,37 +288,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) tile_tab[0] = 0;
   }
   tc_fence_before();
-  __syncthreads();
+  if (kPair)
+    cluster_sync_all();  // both CTAs' barriers and TMEM are there
+  else
+    __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t sf_col0 = p.acc_bufs * p.tn;
   const Table tab{row_tab, blk_tab, tile_tab};
   const int total = tile_tab[p.experts];
   // Work of this CTA: tiles t0, t0 + step, .., K tiles [k0, k1) of each.
-  const int t0 = kSplit ? blockIdx.x / p.splits : blockIdx.x;
-  const int step = kSplit ? total : gridDim.x;  // kSplit: one tile per cluster
-  const int rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int t0 = kSplit ? blockIdx.x / p.splits : kPair ? blockIdx.x >> 1 : blockIdx.x;
+  const int step = kSplit ? total : kPair ? gridDim.x >> 1 : gridDim.x;  // kSplit: one tile per cluster
+  const int rank = kMode == kWhole ? 0 : static_cast<int>(cluster_ctarank());
+  // First feature of this CTA's weight rows.
+  auto feature0 = [&](const Tile& o) { return kPair ? (2 * o.ft + rank) * kF : o.ft * kF; };
   const int k0 = kSplit ? rank * KT / p.splits : 0, k1 = kSplit ? (rank + 1) * KT / p.splits : KT;
   bool partial_ready = false;  // epilogue threads, kSplit: this CTA's partial sums are in TMEM
 
   const int producer = warp == 0 ? 0 : warp >= 10 ? warp - 9 : -1;
   if (producer >= 0) {
     // ------------------------------------------------------------ producers
+    // K tile g of this CTA's sequence (over all its tiles) goes to producer
+    // g % producers, in stage g % S; counters instead of remainders, whose
+    // divisions took longer than the copies.
     if (lane == 0 && producer < p.producers) {
       const uint64_t keep = policy_evict_last(), once = policy_evict_first();
-      int g = 0, e = 0;
+      const int P = p.producers;
+      int e = 0, stage = producer, ahead = producer;  // ahead: this producer's next K tile, counted from the tile's first
+      uint32_t phase = 1;
       const int wblocks = (p.N + 127) >> 7;
       for (int t = t0; t < total && !abort_flag; t += step) {
         const Tile o = tile_at(p, tab, t, e);
-        const int f0 = o.ft * kF;
-        const int64_t wsf = (static_cast<int64_t>(o.e) * wblocks + (f0 >> 7)) * K128 * 512;
+        const int f0 = feature0(o);
+        // (The second CTA's rows may all lie past N: any block's scales do.)
+        const int64_t wsf = (static_cast<int64_t>(o.e) * wblocks + min(f0 >> 7, wblocks - 1)) * K128 * 512;
         const uint8_t* xsf = p.sfx + static_cast<int64_t>(o.blk) * K128 * 512;
         const int nb = ((o.in_blk + o.rows - 1) >> 7) + 1;
-        const int boxes = (o.rows + p.box - 1) / p.box;
-        for (int kt = k0; kt < k1; ++kt, ++g) {
-          if (g % p.producers != producer) continue;
-          const int stage = g % S;
-          if (!mbar_wait(&empty[stage], ((g / S) & 1) ^ 1)) {
+        // The tile's tokens, or this CTA's half of the columns that the MMA
+        // takes: in one box, or in small ones where that would read much more.
+        const int half = ((o.rows + 31) & ~31) >> 1;
+        const int x0 = kPair ? o.row0 + rank * half : o.row0;
+        const int need = kPair ? half : o.rows, small = (need + kSmallBox - 1) / kSmallBox;
+        const bool one_box = 4 * need > 3 * x_rows || small == 1;
+        const CUtensorMap* map_x = 4 * need > 3 * x_rows ? &tm_x : &tm_xs;
+        const uint32_t box_bytes = (4 * need > 3 * x_rows ? x_rows : kSmallBox) * kBKBytes;
+        const int boxes = one_box ? 1 : small;
+        // A pair's loads all complete on the first CTA's barrier.
+        const uint32_t tx = (kABytes + boxes * box_bytes) * (kPair ? 2 : 1);
+        int kt = k0 + ahead;
+        for (; kt < k1; kt += P) {
+          if (!mbar_wait(&empty[stage], phase)) {
             set_status(p.status, kStatusTimeoutEmpty);
             abort_flag = 1;
             break;
@@ -311,81 +352,118 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int b = 0; b < nb; ++b)
             bulk_load(sf + (kSfW + b) * kSfBytes, xsf + (static_cast<int64_t>(b) * K128 + 2 * kt) * 512, bytes,
                       &sf_full[stage], keep);
-          mbar_arrive_expect_tx(&full[stage], kABytes + boxes * p.box * kBKBytes);
+          const uint32_t bar0 = kPair ? map_peer(smem_u32(&full[stage]), 0) : 0;
+          if (!kPair || rank == 0) mbar_arrive_expect_tx(&full[stage], tx);
+          auto load = [&](uint8_t* dst, const CUtensorMap* map, int y, int z, uint64_t policy) {
+            if (kPair)
+              tma_load_3d_pair(dst, map, bar0, kt * kBKBytes, y, z, policy);
+            else
+              tma_load_3d(dst, map, &full[stage], kt * kBKBytes, y, z, policy);
+          };
           if (!(p.inject && blockIdx.x == 0 && t == t0 && kt == k0)) {
-            tma_load_3d(st, &tm_w, &full[stage], kt * kBKBytes, f0, o.e, once);
-            if (kGate) tma_load_3d(st + kABytes / 2, &tm_w2, &full[stage], kt * kBKBytes, f0, o.e, once);
+            load(st, &tm_w, f0, o.e, once);
+            if (kGate) load(st + kABytes / 2, &tm_w2, f0, o.e, once);
           }
-          for (int b = 0; b < boxes; ++b)
-            tma_load_3d(st + kABytes + b * p.box * kBKBytes, &tm_x, &full[stage], kt * kBKBytes, o.row0 + b * p.box, 0,
-                        keep);
+          for (int b = 0; b < boxes; ++b) load(st + kABytes + b * box_bytes, map_x, x0 + b * kSmallBox, 0, keep);
+          stage += P;
+          if (stage >= S) {
+            stage -= S;
+            phase ^= 1;
+          }
         }
+        ahead = kt - k1;
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // ------------------------------------------------------------ MMA issuer (of a pair: the first CTA's)
+    // The whole warp walks the loop and one lane issues: with every operand
+    // uniform over the warp the compiler keeps the descriptors in uniform
+    // registers.  (Inside a one-lane branch each tcgen05.mma cost ~125 cycles of
+    // moves, 800 per K tile, more than its 4 MMAs take.)
+    if (!kPair || rank == 0) {
+      const bool issue = elect_one();
+      const int tiles = __shfl_sync(0xffffffffu, total, 0);
+      const uint64_t desc0 = desc_kmajor_sw128(__shfl_sync(0xffffffffu, smem_u32(smem), 0));
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t sf0 = tmem + sf_col0;
+      const int tail = (p.K - (KT - 1) * kBK + 63) >> 6;  // MMAs of the last K tile
       int stage = 0, acc = 0, e = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = t0; t < total && ok && !abort_flag; t += step) {
-        const Tile o = tile_at(p, tab, t, e);
-        const int n = (o.rows + 31) & ~31;
-        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1)) {
-          set_status(p.status, kStatusTimeoutAccEmpty);
+      for (int t = t0; t < tiles && ok; t += step) {
+        const int n = __shfl_sync(0xffffffffu, (tile_at(p, tab, t, e).rows + 31) & ~31, 0);
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1))) {
+          if (issue) set_status(p.status, kStatusTimeoutAccEmpty);
           abort_flag = 1;
           break;
         }
         tc_fence_after();
-        const uint32_t d = tmem_base + acc * p.tn;
+        const uint32_t d = tmem + acc * p.tn;
+        const uint32_t id0 = idesc_mxf4(kPair ? 2 * kBM : kBM, n, 0), id2 = idesc_mxf4(kPair ? 2 * kBM : kBM, n, 2);
         for (int kt = k0; kt < k1; ++kt) {
-          if (!mbar_wait(&full[stage], phase)) {
-            set_status(p.status, kStatusTimeoutFull);
+          if (!__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(&full[stage], phase) : mbar_wait(&full[stage], phase))) {
+            if (issue) set_status(p.status, kStatusTimeoutFull);
             abort_flag = 1;
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + stage * stage_bytes);
-          const uint32_t sfw = tmem_base + sf_col0 + stage * p.sf_cols, sfx = sfw + 8;
-          const int steps = min(4, (p.K - kt * kBK + 63) >> 6);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            if (kk < steps)
-              mma_mxf4(d, desc_kmajor_sw128(st + kk * 32), desc_kmajor_sw128(st + kABytes + kk * 32),
-                       idesc_mxf4(n, (kk & 1) * 2), sfw + 4 * (kk >> 1), sfx + 4 * p.nblk * (kk >> 1),
-                       kt != k0 || kk != 0);
-          tc_commit(&empty[stage]);
+          const uint64_t a = desc0 + static_cast<uint32_t>(stage * stage_bytes >> 4), b = a + (kABytes >> 4);
+          const uint32_t sfw = sf0 + stage * p.sf_cols, sfx = sfw + 8, more = 4 * p.nblk;
+          const int steps = kt == KT - 1 ? tail : 4;
+          if (issue) {
+            mma_mxf4<kPair>(d, a, b, id0, sfw, sfx, kt != k0);
+            if (steps > 1) mma_mxf4<kPair>(d, a + 2, b + 2, id2, sfw, sfx, 1);
+            if (steps > 2) mma_mxf4<kPair>(d, a + 4, b + 4, id0, sfw + 4, sfx + more, 1);
+            if (steps > 3) mma_mxf4<kPair>(d, a + 6, b + 6, id2, sfw + 4, sfx + more, 1);
+            if (kPair)
+              tc_commit_pair_mc(&empty[stage], 0x3);
+            else
+              tc_commit(&empty[stage]);
+          }
+          __syncwarp();
           if (++stage == S) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        tc_commit(&acc_full[acc]);
+        if (issue) {
+          if (kPair)
+            tc_commit_pair_mc(&acc_full[acc], 0x3);
+          else
+            tc_commit(&acc_full[acc]);
+        }
+        __syncwarp();
         if (++acc == p.acc_bufs) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
       // Every tcgen05 operation has retired before TMEM is freed.
-      tc_commit(drain);
-      mbar_wait(drain, 0);
+      if (issue) {
+        if (kPair)
+          tc_commit_pair(drain);
+        else
+          tc_commit(drain);
+        mbar_wait(drain, 0);
+      }
+      __syncwarp();
     }
   } else if (warp >= 6) {
     // ------------------------------------------------------------ scale writers
-    // Warp 6 + i writes lane quarter (6 + i) % 4.  Per 128 columns of K: the
-    // weight block at columns 4 * kb, the token blocks at 8 + 4 * nblk * kb;
-    // column c of an operand holds the words of its rows 32 c .. 32 c + 31.
+    // Warp 6 + i writes lane quarter (6 + i) % 4.  Columns of a stage: the
+    // weights' two blocks of 128 K columns (4 TMEM columns each), then the
+    // tokens' (4 * nblk each); column c of an operand holds the words of its rows
+    // 32 c .. 32 c + 31.
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
     int stage = 0, e = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int t = t0; t < total && ok; t += step) {
       const Tile o = tile_at(p, tab, t, e);
-      const int nb = ((o.in_blk + o.rows - 1) >> 7) + 1;
       const int shift = o.in_blk >> 5;
-      const int half = ((o.ft * kF) & 127) >> 5;  // gated: the tile's first word in its weight blocks
+      const int half = (feature0(o) & 127) >> 5;  // gated: the tile's first word in its weight blocks
       for (int kt = k0; kt < k1; ++kt) {
         const bool got = mbar_wait(&sf_full[stage], phase);
         if (!__all_sync(0xffffffffu, got && !abort_flag)) {
@@ -397,43 +475,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint8_t* sf = sfbuf + stage * sf_bytes + lane * 16;
         const uint32_t col = tmem_base + quarter + sf_col0 + stage * p.sf_cols;
+        // (Blocks that were not loaded give words of columns that nobody reads.)
+        uint32_t w[8], x[2][8];
+        if (kGate) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint2 v = *reinterpret_cast<const uint2*>(sf + h * kSfBytes + kb * 512 + half * 4);
+              w[4 * kb + 2 * h] = v.x;
+              w[4 * kb + 2 * h + 1] = v.y;
+            }
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) put4(w + 4 * kb, sf + kb * 512);
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          const int left = (p.K >> 5) - 4 * (2 * kt + kb);  // scales per row from here on
-          if (left <= 0) break;
+          put4(x[kb], sf + kSfW * kSfBytes + kb * 512);
+          if (p.nblk > 1)
+            put4(x[kb] + 4, sf + (kSfW + 1) * kSfBytes + kb * 512);
+          else
+#pragma unroll
+            for (int i = 4; i < 8; ++i) x[kb][i] = 0;
+        }
+        const int left = (p.K >> 5) - 8 * kt;  // scales per row from this K tile on
+        if (left < 8) {
           // Padding columns are not the caller's to fill: read as 2^-127.
-          const uint32_t mask = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
-          uint4 v;
-          if (kGate) {
-            const uint2 v1 = *reinterpret_cast<const uint2*>(sf + kb * 512 + half * 4);
-            const uint2 v2 = *reinterpret_cast<const uint2*>(sf + kSfBytes + kb * 512 + half * 4);
-            v = make_uint4(v1.x, v1.y, v2.x, v2.y);
-          } else {
-            v = *reinterpret_cast<const uint4*>(sf + kb * 512);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int n = left - 4 * kb;
+            const uint32_t mask = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * kb + i] &= mask;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[kb][i] &= mask;
           }
-          tmem_st_32x32b_x4(col + 4 * kb, make_uint4(v.x & mask, v.y & mask, v.z & mask, v.w & mask));
-          const uint8_t* xs = sf + kSfW * kSfBytes + kb * 512;
-          uint4 a = *reinterpret_cast<const uint4*>(xs);
-          uint4 b = nb > 1 ? *reinterpret_cast<const uint4*>(xs + kSfBytes) : make_uint4(0, 0, 0, 0);
-          a = make_uint4(a.x & mask, a.y & mask, a.z & mask, a.w & mask);
-          b = make_uint4(b.x & mask, b.y & mask, b.z & mask, b.w & mask);
-          if (shift == 1) {
-            a = make_uint4(a.y, a.z, a.w, b.x);
-            b = make_uint4(b.y, b.z, b.w, 0);
-          } else if (shift == 2) {
-            a = make_uint4(a.z, a.w, b.x, b.y);
-            b = make_uint4(b.z, b.w, 0, 0);
-          } else if (shift == 3) {
-            a = make_uint4(a.w, b.x, b.y, b.z);
-            b = make_uint4(b.w, 0, 0, 0);
-          }
-          tmem_st_32x32b_x4(col + 8 + 4 * p.nblk * kb, a);
-          if (p.nblk > 1) tmem_st_32x32b_x4(col + 8 + 4 * p.nblk * kb + 4, b);
+        }
+        if (shift & 1) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[kb][i] = i < 7 ? x[kb][i + 1] : 0;
+        }
+        if (shift & 2) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[kb][i] = i < 6 ? x[kb][i + 2] : 0;
+        }
+        if (p.nblk > 1) {
+          tmem_st_32x32b_x8(col, w);
+          tmem_st_32x32b_x16(col + 8, x[0], x[1]);
+        } else {
+          const uint32_t both[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+          tmem_st_32x32b_x16(col, w, both);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[stage]);
+        // (Relaxed: the stores are complete and fenced; a release at cluster
+        // scope costs over a thousand cycles.)
+        if (lane == 0) {
+          if (kPair)
+            mbar_arrive_cluster_relaxed(map_peer(smem_u32(&full[stage]), 0));
+          else
+            mbar_arrive(&full[stage]);
+        }
         if (++stage == S) {
           stage = 0;
           phase ^= 1;
@@ -521,9 +629,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         if (c0 + kChunk >= o.rows) {
           tc_fence_before();
-          mbar_arrive(&acc_empty[acc]);
+          if (kPair)
+            mbar_arrive_cluster_relaxed(map_peer(smem_u32(&acc_empty[acc]), 0));
+          else
+            mbar_arrive(&acc_empty[acc]);
         }
-        emit(std::integral_constant<int, 32>(), r, o.row0 + c0, o.ft * kF, min(kChunk, o.rows - c0));
+        emit(std::integral_constant<int, 32>(), r, o.row0 + c0, feature0(o), min(kChunk, o.rows - c0));
       }
       if (++acc == p.acc_bufs) {
         acc = 0;
@@ -582,17 +693,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
             r[4 * h + 3] = __float_as_uint(__uint_as_float(r[4 * h + 3]) + v.w);
           }
-        emit(std::integral_constant<int, 8>(), r, o.row0 + 8 * g, o.ft * kF, min(8, o.rows - 8 * g));
+        emit(std::integral_constant<int, 8>(), r, o.row0 + 8 * g, feature0(o), min(8, o.rows - 8 * g));
       }
     }
   }
 
+  // A pair's MMAs read both CTAs' shared memory and write both TMEMs: neither
+  // CTA leaves before both are done.
   tc_fence_before();
-  __syncthreads();
+  if (kPair)
+    cluster_sync_all();
+  else
+    __syncthreads();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
-    tmem_dealloc(tmem_base, kTmemCols);
+    if (kPair)
+      tmem_dealloc_pair(tmem_base, kTmemCols);
+    else
+      tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
@@ -602,38 +721,42 @@ size_t fixed_smem(int out_size, bool gate, int experts) {
          (3 * kMaxStages + 6) * 8 + 8 + 3 * (static_cast<size_t>(experts) + 1) * 4;
 }
 
-template <typename OutT, bool kGate, bool kSplit>
+template <typename OutT, bool kGate, Mode kMode>
 cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream, const char** why) {
   static bool attr_done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
-  auto kernel = mx_gemm_kernel<OutT, kGate, kSplit>;
+  auto kernel = mx_gemm_kernel<OutT, kGate, kMode>;
   if (dev >= 64 || !attr_done[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_done[dev] = true;
   }
-  CUtensorMap tw, tw2, tx;
+  CUtensorMap tw, tw2, tx, txs;
   const uint64_t k2 = g.K / 2, n = g.N;
   const uint32_t wbox = kGate ? 64 : 128;
   if (!make_tma_3d_u8(&tw, g.b, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox) ||
       (kGate && !make_tma_3d_u8(&tw2, g.b2, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox)) ||
-      !make_tma_3d_u8(&tx, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, p.box)) {
+      !make_tma_3d_u8(&tx, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kMode == kPairs ? p.tn / 2 : p.tn) ||
+      !make_tma_3d_u8(&txs, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kSmallBox)) {
     *why = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kSplit ? p.splits : 1, tw, kGate ? tw2 : tw, tx,
-                    p);
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kMode == kSplitK ? p.splits : kMode == kPairs ? 2 : 1, tw, kGate ? tw2 : tw, tx,
+                    txs, p);
 }
 
 template <typename OutT>
 cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream,
                        const char** why) {
   if (p.splits > 1)
-    return g.b2 ? launch<OutT, true, true>(g, p, smem, grid, stream, why)
-                : launch<OutT, false, true>(g, p, smem, grid, stream, why);
-  return g.b2 ? launch<OutT, true, false>(g, p, smem, grid, stream, why)
-              : launch<OutT, false, false>(g, p, smem, grid, stream, why);
+    return g.b2 ? launch<OutT, true, kSplitK>(g, p, smem, grid, stream, why)
+                : launch<OutT, false, kSplitK>(g, p, smem, grid, stream, why);
+  if (p.pair)
+    return g.b2 ? launch<OutT, true, kPairs>(g, p, smem, grid, stream, why)
+                : launch<OutT, false, kPairs>(g, p, smem, grid, stream, why);
+  return g.b2 ? launch<OutT, true, kWhole>(g, p, smem, grid, stream, why)
+              : launch<OutT, false, kWhole>(g, p, smem, grid, stream, why);
 }
 
 }  // namespace
@@ -655,20 +778,22 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.status = g.status;
   p.inject = g.inject;
   p.vec = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
-  p.n_tiles = (g.N + (gate ? 63 : 127)) / (gate ? 64 : 128);
   // Tokens per tile: the smallest that holds an average expert's rows with
   // room for an uneven routing (an expert over the tile reads its weights twice).
   const int busy = g.experts < g.rows ? g.experts : g.rows;
   const int avg = (g.rows + busy - 1) / busy;
   const int want = g.offsets ? avg + avg / 2 : avg;
   p.tn = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 192;
-  p.box = p.tn < 64 ? p.tn : 64;
+  p.pair = p.tn == 192;
+  const int features = (gate ? 64 : 128) * (p.pair ? 2 : 1);
+  p.n_tiles = (g.N + features - 1) / features;
+  const int x_rows = p.pair ? p.tn / 2 : p.tn;  // token rows in a CTA's shared memory
   p.nblk = p.tn <= 128 ? 1 : 2;
   p.acc_bufs = p.tn <= 192 ? 2 : 1;
   p.sf_cols = 8 + 8 * p.nblk;
   // Stages: what shared memory and TMEM hold.
   const size_t fixed = fixed_smem(out_size, gate, g.experts);
-  const size_t stage = kABytes + p.tn * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;
+  const size_t stage = kABytes + x_rows * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;
   int stages = static_cast<int>((kSmemMax - fixed) / stage);
   const int tmem_stages = (kTmemCols - p.acc_bufs * p.tn) / p.sf_cols;
   stages = stages < tmem_stages ? stages : tmem_stages;
@@ -681,9 +806,10 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const int64_t exact = g.offsets ? tiles : static_cast<int64_t>((g.rows + p.tn - 1) / p.tn) * p.n_tiles;
   const int KT = (g.K + kBK - 1) / kBK;
   p.splits = 1;
-  if (p.tn <= 128)
+  if (!p.pair && p.tn <= 128)
     while (p.splits < 8 && exact * p.splits * 2 <= num_sms && KT >= p.splits * 4) p.splits *= 2;
-  const int64_t grid = p.splits > 1 ? exact * p.splits : exact < num_sms ? exact : num_sms;
+  const int64_t workers = p.pair ? num_sms / 2 : num_sms;
+  const int64_t grid = p.splits > 1 ? exact * p.splits : (exact < workers ? exact : workers) * (p.pair ? 2 : 1);
   const size_t smem = fixed + p.stages * stage;
   return g.out_dtype == 0   ? launch_out<__half>(g, p, smem, static_cast<int>(grid), stream, why)
          : g.out_dtype == 1 ? launch_out<__nv_bfloat16>(g, p, smem, static_cast<int>(grid), stream, why)

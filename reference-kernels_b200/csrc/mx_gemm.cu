@@ -15,11 +15,11 @@
 // A gated tile is 64 rows of b1 over 64 rows of b2, so that both products of
 // an output share a tile, its token operand and its accumulator.
 //
-// One persistent CTA per SM, 13 warps:
+// One persistent CTA per SM, 21 warps:
 //   0, 10..12  TMA producers (K tiles of 256 dealt round-robin)
 //   1          TMEM owner, MMA issuer: tcgen05.mma kind::mxf4 block32, K = 64
-//   2..5       epilogue
-//   6..9       scale writers: each tile's 128x4 scale blocks from shared memory
+//   2..5, 13..16  epilogue: two groups of four, alternate steps of 32 tokens
+//   6..9, 17..20  scale writers, two sets for alternate K tiles: each tile's 128x4 scale blocks from shared memory
 //              to TMEM (tcgen05.st; tcgen05.cp would take tensor-pipe time).  A
 //              token tile that begins inside a block of 128 takes its words from
 //              the block's middle on.
@@ -50,7 +50,9 @@ constexpr int kBKBytes = kBK / 2;
 constexpr int kABytes = kBM * kBKBytes;  // weight bytes per stage
 constexpr int kSfBytes = 1024;           // scales of 128 rows of one stage: two 512-byte blocks
 constexpr int kMaxProducers = 4;
-constexpr int kThreads = 416;
+constexpr int kThreads = 672;
+constexpr int kGroups = 2;               // epilogue groups of four warps
+constexpr int kWriterSets = 2;
 constexpr int kMaxStages = 10;
 constexpr int kTmemCols = 512;
 constexpr int kChunk = 32;               // tokens per epilogue step
@@ -68,6 +70,7 @@ struct Params {
   int tn;         // tokens per tile: 32, 64, 128, 192 or 256
   int nblk;       // 128-row scale blocks that a token tile can touch
   int stages, producers, acc_bufs;
+  int x_cols;     // TMEM columns of the token scales of 128 K columns
   int sf_cols;    // TMEM columns of scales per stage
   int n_tiles;    // tiles along N
   int splits;     // CTAs of a cluster that share a tile's K (kSplitK)
@@ -109,11 +112,50 @@ __device__ __forceinline__ uint32_t idesc_mxf4(int m, int n, uint32_t scale_id) 
          (static_cast<uint32_t>(m >> 4) << 24) | (scale_id << 4) | (scale_id << 29);
 }
 
-__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+// 16 lanes x 8 (32) columns in the layout of an MMA's accumulator: thread t gets
+// of each 8 columns (lane t / 4, columns 2 (t % 4), + 1) and the same of lane
+// t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_16x256b_x1(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(taddr)
                : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// kN 8x8 matrices of 16-bit values, stored transposed: lane l gives the address
+// of row l % 8 of matrix l / 8.
+template <int kN>
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, const uint32_t* v) {
+  if constexpr (kN == 4)
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+  else
+    asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(v[0]), "r"(v[1])
+                 : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// AND of `pred` over the 128 threads of an epilogue group.
+__device__ __forceinline__ bool group_all(int id, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %2, 0;\n\t"
+      "bar.red.and.pred p, %1, 128, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(out)
+      : "r"(id), "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return out != 0;
 }
 
 __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -166,6 +208,16 @@ template <>
 __device__ __forceinline__ float round_to<float>(float v) {
   return v;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t round_pair(uint32_t lo, uint32_t hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 
 // The experts' rows, scale blocks and tiles, in shared memory: E + 1 ints each.
 struct Table {
@@ -204,6 +256,14 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Table& tab, int t
   return o;
 }
 
+// Elements from one token to the next in the epilogue's shared memory: 16 bytes
+// more than the features, so that the eight 16-byte rows of a stored matrix lie
+// in different banks.
+template <typename OutT, bool kGate>
+__host__ __device__ constexpr int staging_pitch() {
+  return (kGate ? 64 : 128) + 16 / sizeof(OutT);
+}
+
 template <typename OutT, bool kGate, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
@@ -219,9 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int stage_bytes = kABytes + x_rows * kBKBytes;
   const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
   uint8_t* sfbuf = smem + S * stage_bytes;
-  OutT* staging = reinterpret_cast<OutT*>(sfbuf + S * sf_bytes);  // two of kChunk x kF
-  float* exch = reinterpret_cast<float*>(staging + 2 * kChunk * kF);  // gated: kChunk x 64
-  uint64_t* bars = reinterpret_cast<uint64_t*>(exch + (kGate ? kChunk * 64 : 0));
+  OutT* staging = reinterpret_cast<OutT*>(sfbuf + S * sf_bytes);  // per group two of kChunk x kPitch
+  constexpr int kPitch = staging_pitch<OutT, kGate>();
+  uint4* exch = reinterpret_cast<uint4*>(staging + kGroups * 2 * kChunk * kPitch);  // gated, per group: 512
+  uint64_t* bars = reinterpret_cast<uint64_t*>(exch + (kGate ? kGroups * 512 : 0));
   uint64_t* full = bars;
   uint64_t* empty = full + S;
   uint64_t* sf_full = empty + S;
@@ -246,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kPair ? 256 : 128);
+      mbar_init(&acc_empty[b], (kPair ? 2 : 1) * kGroups * 128);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
@@ -306,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int k0 = kSplit ? rank * KT / p.splits : 0, k1 = kSplit ? (rank + 1) * KT / p.splits : KT;
   bool partial_ready = false;  // epilogue threads, kSplit: this CTA's partial sums are in TMEM
 
-  const int producer = warp == 0 ? 0 : warp >= 10 ? warp - 9 : -1;
+  const int producer = warp == 0 ? 0 : warp >= 10 && warp <= 12 ? warp - 9 : -1;
   if (producer >= 0) {
     // ------------------------------------------------------------ producers
     // K tile g of this CTA's sequence (over all its tiles) goes to producer
@@ -409,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           const uint64_t a = desc0 + static_cast<uint32_t>(stage * stage_bytes >> 4), b = a + (kABytes >> 4);
-          const uint32_t sfw = sf0 + stage * p.sf_cols, sfx = sfw + 8, more = 4 * p.nblk;
+          const uint32_t sfw = sf0 + stage * p.sf_cols, sfx = sfw + 8, more = p.x_cols;
           const int steps = kt == KT - 1 ? tail : 4;
           if (issue) {
             mma_mxf4<kPair>(d, a, b, id0, sfw, sfx, kt != k0);
@@ -450,21 +511,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-  } else if (warp >= 6) {
+  } else if ((warp >= 6 && warp <= 9) || warp >= 17) {
     // ------------------------------------------------------------ scale writers
-    // Warp 6 + i writes lane quarter (6 + i) % 4.  Columns of a stage: the
+    // Two sets of four warps take alternate K tiles: one set's chain of wait, load,
+    // store and arrival took ~540 cycles a K tile, more than the MMAs.  Warp i
+    // writes lane quarter i % 4.  Columns of a stage: the
     // weights' two blocks of 128 K columns (4 TMEM columns each), then the
-    // tokens' (4 * nblk each); column c of an operand holds the words of its rows
+    // tokens' (x_cols each); column c of an operand holds the words of its rows
     // 32 c .. 32 c + 31.
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    int stage = 0, e = 0;
+    int e = 0, stage = warp >= 17 ? 1 : 0, ahead = stage;  // ahead: this set's next K tile, counted from the tile's first
     uint32_t phase = 0;
     bool ok = true;
     for (int t = t0; t < total && ok; t += step) {
       const Tile o = tile_at(p, tab, t, e);
       const int shift = o.in_blk >> 5;
       const int half = (feature0(o) & 127) >> 5;  // gated: the tile's first word in its weight blocks
-      for (int kt = k0; kt < k1; ++kt) {
+      int kt = k0 + ahead;
+      for (; kt < k1; kt += kWriterSets) {
         const bool got = mbar_wait(&sf_full[stage], phase);
         if (!__all_sync(0xffffffffu, got && !abort_flag)) {
           if (lane == 0 && !got) set_status(p.status, kStatusTimeoutFull);
@@ -524,9 +588,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[kb][i] = i < 6 ? x[kb][i + 2] : 0;
         }
-        if (p.nblk > 1) {
+        if (p.x_cols == 8) {
           tmem_st_32x32b_x8(col, w);
           tmem_st_32x32b_x16(col + 8, x[0], x[1]);
+        } else if (p.x_cols == 6) {
+          const uint32_t some[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[0][4], x[0][5], x[1][0], x[1][1]};
+          tmem_st_32x32b_x16(col, w, some);
+          tmem_st_32x32b_x4(col + 16, make_uint4(x[1][2], x[1][3], x[1][4], x[1][5]));
         } else {
           const uint32_t both[8] = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
           tmem_st_32x32b_x16(col, w, both);
@@ -542,78 +610,126 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             mbar_arrive(&full[stage]);
         }
-        if (++stage == S) {
-          stage = 0;
+        stage += kWriterSets;
+        if (stage >= S) {
+          stage -= S;
           phase ^= 1;
         }
       }
+      ahead = kt - k1;
     }
   }
 
   // ------------------------------------------------------------ epilogue
-  const bool epi = warp >= 2 && warp <= 5;
-  const int q = warp & 3;
-  const int rloc = q * 32 + lane;  // TMEM lane: the tile's weight row
+  const int group = warp >= 2 && warp <= 5 ? 0 : warp >= 13 && warp <= 16 ? 1 : -1;
+  const int q = warp & 3;                       // lane quarter: weight rows 32 q .. 32 q + 31
+  const int gtid = (warp < 6 ? warp - 2 : warp - 13) * 32 + lane;  // thread of the group
   const uint32_t tquarter = static_cast<uint32_t>(q * 32) << 16;
   OutT* const c = static_cast<OutT*>(p.c);
-  // W tokens (columns) of this thread's weight row to rows row0 .. of C, features
-  // f0 ..; `valid` tokens are stored.  Through shared memory, where a token's
-  // features lie together: 2-byte stores of a warp's 32 features side by side,
-  // then 16 bytes per thread.
+  // This warp's 32 weight rows x 8 G tokens in r[half][4 G] (the two halves of
+  // its rows, as tcgen05.ld 16x256b leaves them) to rows row0 .. of C, features
+  // f0 ..; `valid` tokens are stored.  The values pass through shared memory,
+  // transposed by stmatrix so that a token's features lie together, and leave in
+  // 16-byte stores.
   int buf = 0;
-  auto emit = [&](auto width, const uint32_t* r, int64_t row0, int f0, int valid) {
-    constexpr int W = decltype(width)::value;
-    OutT* out = staging + buf * kChunk * kF;
+  auto emit = [&](auto width, uint32_t* r, int64_t row0, int f0, int valid) {
+    constexpr int G = decltype(width)::value, kR = 4 * G;
+    constexpr int kHalves = kGate && G == 1 ? 1 : 2;       // row halves that this warp computes
+    constexpr int kTok = kGate && G > 1 ? G / 2 : G;       // its groups of 8 tokens
+    OutT* out = staging + (group * 2 + buf) * kChunk * kPitch;
     buf ^= 1;
+    int feature = q * 32, token = 0;  // of what this warp computes
     if (kGate) {
-      // Lanes 0..63 hold x1, 64..127 x2 of the same outputs: each half gives the
-      // other one half of the tokens and computes the rest.
-      const bool first = rloc < 64;
-      const int f = rloc & 63;
-      float* const give = exch + (first ? W / 2 : 0) * 64 + f;
-      const float* const take = exch + (first ? 0 : W / 2) * 64 + f;
-      OutT* const dst = out + (first ? 0 : W / 2) * kF + f;
+      // Warps 0 and 1 of a group hold x1, 2 and 3 x2 of the same outputs: each
+      // gives its partner half of its values (half of the tokens, or of 8 tokens
+      // half of the rows) and computes the other half.
+      const bool first = q < 2;
+      uint4* const box = exch + group * 512 + (q & 1) * 256 + lane;
+      constexpr int kV = kR / 4;  // 16-byte vectors given
+      // Values given and kept, as r indices: G > 1: token groups; G == 1: row halves.
+      auto at = [&](bool upper, int i) {
+        return G == 1 ? (upper ? kR : 0) + i : (i / (kR / 2)) * kR + (upper ? kR / 2 : 0) + i % (kR / 2);
+      };
+      uint32_t keep[kR];
 #pragma unroll
-      for (int i = 0; i < W / 2; ++i) give[i * 64] = __uint_as_float(first ? r[W / 2 + i] : r[i]);
-      epi_bar();
+      for (int v = 0; v < kV; ++v) {
+        uint32_t g[4];
 #pragma unroll
-      for (int i = 0; i < W / 2; ++i) {
-        const float own = __uint_as_float(first ? r[i] : r[W / 2 + i]), other = take[i * 64];
-        dst[i * kF] = round_to<OutT>(silu_mul(first ? own : other, first ? other : own));
+        for (int i = 0; i < 4; ++i) {
+          g[i] = first ? r[at(true, 4 * v + i)] : r[at(false, 4 * v + i)];
+          keep[4 * v + i] = first ? r[at(false, 4 * v + i)] : r[at(true, 4 * v + i)];
+        }
+        box[(first ? 0 : 128) + v * 32] = make_uint4(g[0], g[1], g[2], g[3]);
       }
-    } else {
+      bar_sync(3 + group * 2 + (q & 1), 64);
 #pragma unroll
-      for (int i = 0; i < W; ++i) out[i * kF + rloc] = round_to<OutT>(__uint_as_float(r[i]));
-    }
-    epi_bar();
-    constexpr int kPer = 16 / sizeof(OutT), kVecs = kF / kPer;
-    const int tid = threadIdx.x - 64;
-    if (p.vec) {
-      for (int i = tid; i < W * kVecs; i += 128) {
-        const int tok = i / kVecs, f = (i % kVecs) * kPer;
-        if (tok >= valid || f0 + f >= p.N) continue;
-        OutT* dst = c + (row0 + tok) * p.ldc + f0 + f;
-        if (f0 + f + kPer <= p.N) {
-          *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out + tok * kF + f);
-        } else {
-          for (int j = 0; f0 + f + j < p.N; ++j) dst[j] = out[tok * kF + f + j];
+      for (int v = 0; v < kV; ++v) {
+        const uint4 o = box[(first ? 128 : 0) + v * 32];
+        const uint32_t other[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = __uint_as_float(first ? keep[4 * v + i] : other[i]);
+          const float y = __uint_as_float(first ? other[i] : keep[4 * v + i]);
+          r[4 * v + i] = __float_as_uint(silu_mul(x, y));
         }
       }
+      feature = (q & 1) * 32 + (G == 1 && !first ? 16 : 0);
+      token = G > 1 && !first ? 8 * kTok : 0;
+    }
+    // r[half][4 kTok] now, kHalves halves.
+    if constexpr (sizeof(OutT) == 2) {
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        uint32_t m[2 * kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          m[2 * h] = round_pair<OutT>(r[h * 4 * kTok + 4 * j], r[h * 4 * kTok + 4 * j + 1]);
+          m[2 * h + 1] = round_pair<OutT>(r[h * 4 * kTok + 4 * j + 2], r[h * 4 * kTok + 4 * j + 3]);
+        }
+        stmatrix_trans<2 * kHalves>(
+            smem_u32(out + (token + 8 * j + (lane & 7)) * kPitch + feature + 8 * ((lane >> 3) & (2 * kHalves - 1))), m);
+      }
     } else {
-      for (int i = tid; i < W * kF; i += 128) {
+#pragma unroll
+      for (int j = 0; j < kTok; ++j)
+#pragma unroll
+        for (int i = 0; i < 4 * kHalves; ++i) {
+          const int h = i >> 2, f = feature + 16 * h + ((i & 2) ? 8 : 0) + (lane >> 2);
+          out[(token + 8 * j + 2 * (lane & 3) + (i & 1)) * kPitch + f] =
+              round_to<OutT>(__uint_as_float(r[h * 4 * kTok + 4 * j + (i & 3)]));
+        }
+    }
+    bar_sync(1 + group, 128);
+    constexpr int kPer = 16 / sizeof(OutT), kVecs = kF / kPer, kStep = 128 / kVecs;
+    if (p.vec) {
+      const int f = (gtid % kVecs) * kPer, t0 = gtid / kVecs;
+      const OutT* src = out + t0 * kPitch + f;
+      OutT* dst = c + (row0 + t0) * p.ldc + f0 + f;
+      const int left = p.N - f0 - f;
+      if (left >= kPer) {
+#pragma unroll
+        for (int i = 0; i < (8 * G + kStep - 1) / kStep; ++i)
+          if (t0 + i * kStep < valid)
+            *reinterpret_cast<uint4*>(dst + i * kStep * p.ldc) = *reinterpret_cast<const uint4*>(src + i * kStep * kPitch);
+      } else {
+        for (int i = t0; i < valid; i += kStep, src += kStep * kPitch, dst += kStep * p.ldc)
+          for (int j = 0; j < left; ++j) dst[j] = src[j];
+      }
+    } else {
+      for (int i = gtid; i < valid * kF; i += 128) {
         const int tok = i / kF, f = i % kF;
-        if (tok < valid && f0 + f < p.N) c[(row0 + tok) * p.ldc + f0 + f] = out[i];
+        if (f0 + f < p.N) c[(row0 + tok) * p.ldc + f0 + f] = out[tok * kPitch + f];
       }
     }
   };
-  if (epi) {
+  if (group >= 0 && (!kSplit || group == 0)) {
     int acc = 0, e = 0;
     uint32_t acc_phase = 0;
     for (int t = t0; t < total; t += step) {
       const Tile o = tile_at(p, tab, t, e);
       // The four warps agree before any goes on to the named barriers.
-      if (!epi_all(mbar_wait(&acc_full[acc], acc_phase))) {
-        if (threadIdx.x == 64) set_status(p.status, kStatusTimeoutAccFull);
+      if (!group_all(1 + group, mbar_wait(&acc_full[acc], acc_phase))) {
+        if (gtid == 0) set_status(p.status, kStatusTimeoutAccFull);
         abort_flag = 1;
         break;
       }
@@ -623,18 +739,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const uint32_t tacc = tmem_base + tquarter + acc * p.tn;
-      for (int c0 = 0; c0 < o.rows; c0 += kChunk) {
+      auto release = [&]() {
+        tc_fence_before();
+        if (kPair)
+          mbar_arrive_cluster_relaxed(map_peer(smem_u32(&acc_empty[acc]), 0));
+        else
+          mbar_arrive(&acc_empty[acc]);
+      };
+      if (group * kChunk >= o.rows) release();
+      for (int c0 = group * kChunk; c0 < o.rows; c0 += kGroups * kChunk) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(tacc + c0, r);
+        tmem_ld_16x256b_x4(tacc + c0, r);
+        tmem_ld_16x256b_x4(tacc + (16u << 16) + c0, r + 16);
         tmem_wait_ld();
-        if (c0 + kChunk >= o.rows) {
-          tc_fence_before();
-          if (kPair)
-            mbar_arrive_cluster_relaxed(map_peer(smem_u32(&acc_empty[acc]), 0));
-          else
-            mbar_arrive(&acc_empty[acc]);
-        }
-        emit(std::integral_constant<int, 32>(), r, o.row0 + c0, feature0(o), min(kChunk, o.rows - c0));
+        if (c0 + kGroups * kChunk >= o.rows) release();
+        emit(std::integral_constant<int, 4>(), r, o.row0 + c0, feature0(o), min(kChunk, o.rows - c0));
       }
       if (++acc == p.acc_bufs) {
         acc = 0;
@@ -642,9 +761,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // Rows that belong to no expert.
-    const int tid = threadIdx.x - 64;
-    for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
-      for (int f = tid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
+    if (group == 0)
+      for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
+        for (int f = gtid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
   }
 
   if (kSplit && t0 < total) {
@@ -653,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // sends its partial sums of the other ranks' shares to their shared memory
     // (the pipeline's, free once every rank is past its main loop) and adds up
     // its own share, own sums first and then by rank: the same order always.
-    const bool ok = epi ? epi_all(partial_ready) : true;
+    const bool epi = group == 0;
+    const bool ok = epi ? group_all(1, partial_ready) : true;
     tc_fence_after();
     cluster_sync_all();
     int e = 0;
@@ -662,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int share = (ng + p.splits - 1) / p.splits;
     const uint32_t tacc = tmem_base + tquarter;
     auto at = [&](int slot, int gi, int half) {
-      return static_cast<uint32_t>((((slot * share + gi) * 2 + half) * kBM + rloc) * 16);
+      return static_cast<uint32_t>((((slot * share + gi) * 2 + half) * 128 + gtid) * 16);
     };
     if (epi && ok) {
       for (int i = 1; i < p.splits; ++i) {
@@ -671,7 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int slot = rank < peer ? rank : rank - 1;
         for (int g = peer * share; g < min(ng, (peer + 1) * share); ++g) {
           uint32_t r[8];
-          tmem_ld_32x32b_x8(tacc + 8 * g, r);
+          tmem_ld_16x256b_x1(tacc + 8 * g, r);
+          tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * g, r + 4);
           tmem_wait_ld();
           st_cluster_v4(base + at(slot, g - peer * share, 0), r);
           st_cluster_v4(base + at(slot, g - peer * share, 1), r + 4);
@@ -682,7 +803,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (epi && ok) {
       for (int g = rank * share; g < min(ng, (rank + 1) * share); ++g) {
         uint32_t r[8];
-        tmem_ld_32x32b_x8(tacc + 8 * g, r);
+        tmem_ld_16x256b_x1(tacc + 8 * g, r);
+        tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * g, r + 4);
         tmem_wait_ld();
         for (int slot = 0; slot < p.splits - 1; ++slot)
 #pragma unroll
@@ -693,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
             r[4 * h + 3] = __float_as_uint(__uint_as_float(r[4 * h + 3]) + v.w);
           }
-        emit(std::integral_constant<int, 8>(), r, o.row0 + 8 * g, feature0(o), min(8, o.rows - 8 * g));
+        emit(std::integral_constant<int, 1>(), r, o.row0 + 8 * g, feature0(o), min(8, o.rows - 8 * g));
       }
     }
   }
@@ -716,9 +838,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 size_t fixed_smem(int out_size, bool gate, int experts) {
-  const int f = gate ? 64 : 128;
-  return 1024 /* alignment */ + 2 * kChunk * f * out_size + (gate ? kChunk * 64 * 4 : 0) +
-         (3 * kMaxStages + 6) * 8 + 8 + 3 * (static_cast<size_t>(experts) + 1) * 4;
+  const int pitch = (gate ? 64 : 128) * out_size + 16;
+  return 1024 /* alignment */ + kGroups * (2 * kChunk * pitch + (gate ? 512 * 16 : 0)) + (3 * kMaxStages + 6) * 8 + 8 + 3 * (static_cast<size_t>(experts) + 1) * 4;
 }
 
 template <typename OutT, bool kGate, Mode kMode>
@@ -790,7 +911,8 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const int x_rows = p.pair ? p.tn / 2 : p.tn;  // token rows in a CTA's shared memory
   p.nblk = p.tn <= 128 ? 1 : 2;
   p.acc_bufs = p.tn <= 192 ? 2 : 1;
-  p.sf_cols = 8 + 8 * p.nblk;
+  p.x_cols = p.tn <= 128 ? 4 : p.tn / 32;
+  p.sf_cols = 8 + 2 * p.x_cols;
   // Stages: what shared memory and TMEM hold.
   const size_t fixed = fixed_smem(out_size, gate, g.experts);
   const size_t stage = kABytes + x_rows * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;
@@ -798,6 +920,12 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const int tmem_stages = (kTmemCols - p.acc_bufs * p.tn) / p.sf_cols;
   stages = stages < tmem_stages ? stages : tmem_stages;
   p.stages = stages < kMaxStages ? stages : kMaxStages;
+  // An even number: a stage then always belongs to the same set of scale
+  // writers.  A set waits for its stage by phase parity, which is exact only if
+  // it has itself seen the stage's previous phase; with an odd number it would
+  // find every other phase waited for by the other set, and could take the one
+  // before that for its own.
+  p.stages &= ~(kWriterSets - 1);
   // A producer waits on a stage by phase parity, which is exact only while it
   // waits for every stage at most one lap behind: not more producers than stages.
   p.producers = p.stages < kMaxProducers ? p.stages : kMaxProducers;

@@ -256,19 +256,25 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Table& tab, int t
   return o;
 }
 
-// Elements from one token to the next in the epilogue's shared memory: 16 bytes
-// more than the features, so that the eight 16-byte rows of a stored matrix lie
-// in different banks.
-template <typename OutT, bool kGate>
-__host__ __device__ constexpr int staging_pitch() {
-  return (kGate ? 64 : 128) + 16 / sizeof(OutT);
+// The epilogue's staging of 32 tokens: boxes of 32 x 128 bytes with the 128-byte
+// swizzle of a TMA store, so that matrices of 8 tokens x 16 bytes and whole rows
+// are both free of bank conflicts.  Byte offset of feature f of token t:
+template <typename OutT>
+__device__ __forceinline__ int staged(int t, int f) {
+  const int b = f * static_cast<int>(sizeof(OutT));
+  return (b >> 7) * (kChunk * 128) + t * 128 + ((b & 112) ^ ((t & 7) << 4)) + (b & 15);
+}
+// Staging buffers per group: 16-bit types write one while the other is stored.
+template <typename OutT>
+__host__ __device__ constexpr int staging_bufs() {
+  return sizeof(OutT) == 2 ? 2 : 1;
 }
 
 template <typename OutT, bool kGate, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
                    const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_xs,
-                   const Params p) {
+                   const __grid_constant__ CUtensorMap tm_c, const Params p) {
   constexpr int kF = kGate ? 64 : 128;  // output features per tile
   constexpr int kSfW = kGate ? 2 : 1;   // weight scale blocks per 128 columns of K
   constexpr bool kSplit = kMode == kSplitK, kPair = kMode == kPairs;
@@ -278,10 +284,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int x_rows = kPair ? p.tn / 2 : p.tn;  // token rows of a stage
   const int stage_bytes = kABytes + x_rows * kBKBytes;
   const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
-  uint8_t* sfbuf = smem + S * stage_bytes;
-  OutT* staging = reinterpret_cast<OutT*>(sfbuf + S * sf_bytes);  // per group two of kChunk x kPitch
-  constexpr int kPitch = staging_pitch<OutT, kGate>();
-  uint4* exch = reinterpret_cast<uint4*>(staging + kGroups * 2 * kChunk * kPitch);  // gated, per group: 512
+  constexpr int kBufs = staging_bufs<OutT>(), kStaged = kChunk * kF * sizeof(OutT);
+  uint8_t* staging = smem + S * stage_bytes;  // per group kBufs of kStaged bytes (1024-aligned)
+  uint8_t* sfbuf = staging + kGroups * kBufs * kStaged;
+  uint4* exch = reinterpret_cast<uint4*>(sfbuf + S * sf_bytes);  // gated, per group: 512
   uint64_t* bars = reinterpret_cast<uint64_t*>(exch + (kGate ? kGroups * 512 : 0));
   uint64_t* full = bars;
   uint64_t* empty = full + S;
@@ -636,8 +642,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int G = decltype(width)::value, kR = 4 * G;
     constexpr int kHalves = kGate && G == 1 ? 1 : 2;       // row halves that this warp computes
     constexpr int kTok = kGate && G > 1 ? G / 2 : G;       // its groups of 8 tokens
-    OutT* out = staging + (group * 2 + buf) * kChunk * kPitch;
-    buf ^= 1;
+    uint8_t* out = staging + (group * kBufs + buf) * kStaged;
+    if (kBufs == 2) {
+      buf ^= 1;
+    } else {  // the buffer's last store has read it
+      if (gtid == 0) bulk_wait_group_read0();
+      bar_sync(1 + group, 128);
+    }
     int feature = q * 32, token = 0;  // of what this warp computes
     if (kGate) {
       // Warps 0 and 1 of a group hold x1, 2 and 3 x2 of the same outputs: each
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m[2 * h + 1] = round_pair<OutT>(r[h * 4 * kTok + 4 * j + 2], r[h * 4 * kTok + 4 * j + 3]);
         }
         stmatrix_trans<2 * kHalves>(
-            smem_u32(out + (token + 8 * j + (lane & 7)) * kPitch + feature + 8 * ((lane >> 3) & (2 * kHalves - 1))), m);
+            smem_u32(out + staged<OutT>(token + 8 * j + (lane & 7), feature + 8 * ((lane >> 3) & (2 * kHalves - 1)))), m);
       }
     } else {
 #pragma unroll
@@ -695,30 +706,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4 * kHalves; ++i) {
           const int h = i >> 2, f = feature + 16 * h + ((i & 2) ? 8 : 0) + (lane >> 2);
-          out[(token + 8 * j + 2 * (lane & 3) + (i & 1)) * kPitch + f] =
+          *reinterpret_cast<OutT*>(out + staged<OutT>(token + 8 * j + 2 * (lane & 3) + (i & 1), f)) =
               round_to<OutT>(__uint_as_float(r[h * 4 * kTok + 4 * j + (i & 3)]));
         }
     }
+    // A whole step, or the last rows of C, in TMA stores; the end of an expert's
+    // rows, and a C whose rows are not 16-byte aligned, by the threads.
+    const bool tma = G == 4 && p.vec && (valid == kChunk || row0 + valid == p.rows);
+    if (tma) fence_proxy_async_smem();
+    if (kBufs == 2 && gtid == 0) bulk_wait_group_read0();  // the other buffer, which the next step writes, is read
     bar_sync(1 + group, 128);
-    constexpr int kPer = 16 / sizeof(OutT), kVecs = kF / kPer, kStep = 128 / kVecs;
-    if (p.vec) {
-      const int f = (gtid % kVecs) * kPer, t0 = gtid / kVecs;
-      const OutT* src = out + t0 * kPitch + f;
-      OutT* dst = c + (row0 + t0) * p.ldc + f0 + f;
-      const int left = p.N - f0 - f;
-      if (left >= kPer) {
+    if (tma) {
+      if (gtid == 0) {
 #pragma unroll
-        for (int i = 0; i < (8 * G + kStep - 1) / kStep; ++i)
-          if (t0 + i * kStep < valid)
-            *reinterpret_cast<uint4*>(dst + i * kStep * p.ldc) = *reinterpret_cast<const uint4*>(src + i * kStep * kPitch);
-      } else {
-        for (int i = t0; i < valid; i += kStep, src += kStep * kPitch, dst += kStep * p.ldc)
-          for (int j = 0; j < left; ++j) dst[j] = src[j];
+        for (int b = 0; b < kStaged / (kChunk * 128); ++b)
+          if (f0 * static_cast<int>(sizeof(OutT)) + b * 128 < p.N * static_cast<int>(sizeof(OutT)))
+            tma_store_3d(&tm_c, out + b * kChunk * 128, f0 * static_cast<int>(sizeof(OutT)) + b * 128,
+                         static_cast<int>(row0), 0);
+        bulk_commit_group();
       }
+    } else if (p.vec) {
+      constexpr int kPer = 16 / sizeof(OutT), kVecs = kF / kPer;
+      const int f = (gtid % kVecs) * kPer;
+      if (f0 + f < p.N)  // (p.vec: N is a multiple of kPer, or ldc is more than N)
+        for (int i = gtid / kVecs; i < valid; i += 128 / kVecs) {
+          const uint8_t* src = out + staged<OutT>(i, f);
+          OutT* dst = c + (row0 + i) * p.ldc + f0 + f;
+          if (f0 + f + kPer <= p.N)
+            *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+          else
+            for (int k = 0; f0 + f + k < p.N; ++k) dst[k] = reinterpret_cast<const OutT*>(src)[k];
+        }
     } else {
       for (int i = gtid; i < valid * kF; i += 128) {
         const int tok = i / kF, f = i % kF;
-        if (f0 + f < p.N) c[(row0 + tok) * p.ldc + f0 + f] = out[tok * kPitch + f];
+        if (f0 + f < p.N) c[(row0 + tok) * p.ldc + f0 + f] = *reinterpret_cast<const OutT*>(out + staged<OutT>(tok, f));
       }
     }
   };
@@ -820,6 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if (group >= 0 && gtid == 0) bulk_wait_group0();  // C is written before the CTA ends
   // A pair's MMAs read both CTAs' shared memory and write both TMEMs: neither
   // CTA leaves before both are done.
   tc_fence_before();
@@ -838,8 +861,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 size_t fixed_smem(int out_size, bool gate, int experts) {
-  const int pitch = (gate ? 64 : 128) * out_size + 16;
-  return 1024 /* alignment */ + kGroups * (2 * kChunk * pitch + (gate ? 512 * 16 : 0)) + (3 * kMaxStages + 6) * 8 + 8 + 3 * (static_cast<size_t>(experts) + 1) * 4;
+  const int staged = kChunk * (gate ? 64 : 128) * out_size * (out_size == 2 ? 2 : 1);
+  return 1024 /* alignment */ + kGroups * (staged + (gate ? 512 * 16 : 0)) + (3 * kMaxStages + 6) * 8 + 8 +
+         3 * (static_cast<size_t>(experts) + 1) * 4;
 }
 
 template <typename OutT, bool kGate, Mode kMode>
@@ -853,18 +877,20 @@ cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, 
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_done[dev] = true;
   }
-  CUtensorMap tw, tw2, tx, txs;
+  CUtensorMap tw, tw2, tx, txs, tc;
   const uint64_t k2 = g.K / 2, n = g.N;
   const uint32_t wbox = kGate ? 64 : 128;
   if (!make_tma_3d_u8(&tw, g.b, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox) ||
       (kGate && !make_tma_3d_u8(&tw2, g.b2, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox)) ||
       !make_tma_3d_u8(&tx, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kMode == kPairs ? p.tn / 2 : p.tn) ||
-      !make_tma_3d_u8(&txs, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kSmallBox)) {
+      !make_tma_3d_u8(&txs, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kSmallBox) ||
+      (p.vec && !make_tma_3d_u8(&tc, g.c, n * sizeof(OutT), g.rows, 1, g.ldc * sizeof(OutT),
+                                g.ldc * sizeof(OutT) * g.rows, 128, kChunk))) {
     *why = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
   return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kMode == kSplitK ? p.splits : kMode == kPairs ? 2 : 1, tw, kGate ? tw2 : tw, tx,
-                    txs, p);
+                    txs, p.vec ? tc : tx, p);
 }
 
 template <typename OutT>

@@ -179,6 +179,35 @@ __device__ __forceinline__ void put4(uint32_t* dst, const uint8_t* src) {
   dst[3] = v.w;
 }
 
+// Shared-memory operands by address (uniform over the warp).
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_load_u32(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
+                                              uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+      : "memory");
+}
+template <bool kTwo>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
+                                          uint64_t policy) {
+  if (kTwo)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+}
+
 // One lane of a converged warp, the same on every call.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -232,6 +261,13 @@ struct Tile {
   int blk;     // its scale block
   int ft;      // tile along N
 };
+
+// The tile in values that the compiler knows to be the same in every lane.
+__device__ __forceinline__ Tile uniform(const Tile& o) {
+  return Tile{__shfl_sync(0xffffffffu, o.e, 0),      __shfl_sync(0xffffffffu, o.row0, 0),
+              __shfl_sync(0xffffffffu, o.rows, 0),   __shfl_sync(0xffffffffu, o.in_blk, 0),
+              __shfl_sync(0xffffffffu, o.blk, 0),    __shfl_sync(0xffffffffu, o.ft, 0)};
+}
 
 // Tile t (< tab.tile[E]); `e` is the walker's cursor.  Tiles of an expert go
 // over up to kGroup token tiles for each weight tile, so that CTAs that run
@@ -379,14 +415,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // K tile g of this CTA's sequence (over all its tiles) goes to producer
     // g % producers, in stage g % S; counters instead of remainders, whose
     // divisions took longer than the copies.
-    if (lane == 0 && producer < p.producers) {
+    // (As the MMA issuer, the whole warp walks and one lane issues.)
+    if (producer < p.producers) {
+      const bool issue = elect_one();
+      const int tiles = __shfl_sync(0xffffffffu, total, 0);
       const uint64_t keep = policy_evict_last(), once = policy_evict_first();
       const int P = p.producers;
       int e = 0, stage = producer, ahead = producer;  // ahead: this producer's next K tile, counted from the tile's first
       uint32_t phase = 1;
       const int wblocks = (p.N + 127) >> 7;
-      for (int t = t0; t < total && !abort_flag; t += step) {
-        const Tile o = tile_at(p, tab, t, e);
+      const uint32_t stages0 = __shfl_sync(0xffffffffu, smem_u32(smem), 0), sf0 = __shfl_sync(0xffffffffu, smem_u32(sfbuf), 0);
+      const uint32_t full0 = __shfl_sync(0xffffffffu, smem_u32(full), 0), sf_full0 = full0 + 16 * S;
+      bool ok = true;
+      for (int t = t0; t < tiles && ok; t += step) {
+        const Tile o = uniform(tile_at(p, tab, t, e));
         const int f0 = feature0(o);
         // (The second CTA's rows may all lie past N: any block's scales do.)
         const int64_t wsf = (static_cast<int64_t>(o.e) * wblocks + min(f0 >> 7, wblocks - 1)) * K128 * 512;
@@ -405,33 +447,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tx = (kABytes + boxes * box_bytes) * (kPair ? 2 : 1);
         int kt = k0 + ahead;
         for (; kt < k1; kt += P) {
-          if (!mbar_wait(&empty[stage], phase)) {
-            set_status(p.status, kStatusTimeoutEmpty);
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase) && !abort_flag)) {
+            if (issue) set_status(p.status, kStatusTimeoutEmpty);
             abort_flag = 1;
+            ok = false;
             break;
           }
-          uint8_t* st = smem + stage * stage_bytes;
-          uint8_t* sf = sfbuf + stage * sf_bytes;
-          const uint32_t bytes = min(2, K128 - 2 * kt) * 512;
-          mbar_arrive_expect_tx(&sf_full[stage], (kSfW + nb) * bytes);
-          bulk_load(sf, p.sfw + wsf + kt * kSfBytes, bytes, &sf_full[stage], once);
-          if (kGate) bulk_load(sf + kSfBytes, p.sfw2 + wsf + kt * kSfBytes, bytes, &sf_full[stage], once);
-          for (int b = 0; b < nb; ++b)
-            bulk_load(sf + (kSfW + b) * kSfBytes, xsf + (static_cast<int64_t>(b) * K128 + 2 * kt) * 512, bytes,
-                      &sf_full[stage], keep);
-          const uint32_t bar0 = kPair ? map_peer(smem_u32(&full[stage]), 0) : 0;
-          if (!kPair || rank == 0) mbar_arrive_expect_tx(&full[stage], tx);
-          auto load = [&](uint8_t* dst, const CUtensorMap* map, int y, int z, uint64_t policy) {
-            if (kPair)
-              tma_load_3d_pair(dst, map, bar0, kt * kBKBytes, y, z, policy);
-            else
-              tma_load_3d(dst, map, &full[stage], kt * kBKBytes, y, z, policy);
-          };
-          if (!(p.inject && blockIdx.x == 0 && t == t0 && kt == k0)) {
-            load(st, &tm_w, f0, o.e, once);
-            if (kGate) load(st + kABytes / 2, &tm_w2, f0, o.e, once);
+          if (issue) {
+            const uint32_t st = stages0 + stage * stage_bytes, sf = sf0 + stage * sf_bytes;
+            const uint32_t bar = full0 + 8 * stage, sf_bar = sf_full0 + 8 * stage;
+            const uint32_t bytes = min(2, K128 - 2 * kt) * 512;
+            expect_tx(sf_bar, (kSfW + nb) * bytes);
+            bulk_load_u32(sf, p.sfw + wsf + kt * kSfBytes, bytes, sf_bar, once);
+            if (kGate) bulk_load_u32(sf + kSfBytes, p.sfw2 + wsf + kt * kSfBytes, bytes, sf_bar, once);
+            bulk_load_u32(sf + kSfW * kSfBytes, xsf + 2 * kt * 512, bytes, sf_bar, keep);
+            if (nb > 1)
+              bulk_load_u32(sf + (kSfW + 1) * kSfBytes, xsf + (static_cast<int64_t>(K128) + 2 * kt) * 512, bytes, sf_bar,
+                            keep);
+            if (!kPair || rank == 0) expect_tx(bar, tx);
+            const uint32_t tile_bar = kPair ? map_peer(bar, 0) : bar;
+            if (!(p.inject && blockIdx.x == 0 && t == t0 && kt == k0)) {
+              load_tile<kPair>(st, &tm_w, tile_bar, kt * kBKBytes, f0, o.e, once);
+              if (kGate) load_tile<kPair>(st + kABytes / 2, &tm_w2, tile_bar, kt * kBKBytes, f0, o.e, once);
+            }
+            for (int b = 0; b < boxes; ++b)
+              load_tile<kPair>(st + kABytes + b * box_bytes, map_x, tile_bar, kt * kBKBytes, x0 + b * kSmallBox, 0, keep);
           }
-          for (int b = 0; b < boxes; ++b) load(st + kABytes + b * box_bytes, map_x, x0 + b * kSmallBox, 0, keep);
+          __syncwarp();
           stage += P;
           if (stage >= S) {
             stage -= S;

@@ -31,6 +31,7 @@
 // partial sums through distributed shared memory, in rank order.
 #include <cuda_bf16.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -786,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   };
-  if (group >= 0 && (!kSplit || group == 0)) {
+  if (group >= 0) {
     int acc = 0, e = 0;
     uint32_t acc_phase = 0;
     for (int t = t0; t < total; t += step) {
@@ -836,8 +837,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // sends its partial sums of the other ranks' shares to their shared memory
     // (the pipeline's, free once every rank is past its main loop) and adds up
     // its own share, own sums first and then by rank: the same order always.
-    const bool epi = group == 0;
-    const bool ok = epi ? group_all(1, partial_ready) : true;
+    // The epilogue groups take the even and the odd ones.
+    const bool ok = group >= 0 ? group_all(1 + group, partial_ready) : true;
     tc_fence_after();
     cluster_sync_all();
     int e = 0;
@@ -848,24 +849,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto at = [&](int slot, int gi, int half) {
       return static_cast<uint32_t>((((slot * share + gi) * 2 + half) * 128 + gtid) * 16);
     };
-    if (epi && ok) {
+    if (group >= 0 && ok) {
+      constexpr int kAtOnce = 4;  // groups whose loads are in flight together
       for (int i = 1; i < p.splits; ++i) {
         const int peer = (rank + i) % p.splits;
         const uint32_t base = map_peer(smem_u32(smem), peer);
         const int slot = rank < peer ? rank : rank - 1;
-        for (int g = peer * share; g < min(ng, (peer + 1) * share); ++g) {
-          uint32_t r[8];
-          tmem_ld_16x256b_x1(tacc + 8 * g, r);
-          tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * g, r + 4);
+        const int first = peer * share, end = min(ng, first + share);
+        for (int g0 = first + ((first ^ group) & 1); g0 < end; g0 += kGroups * kAtOnce) {
+          uint32_t r[kAtOnce][8];
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k)
+            if (g0 + kGroups * k < end) {
+              tmem_ld_16x256b_x1(tacc + 8 * (g0 + kGroups * k), r[k]);
+              tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * (g0 + kGroups * k), r[k] + 4);
+            }
           tmem_wait_ld();
-          st_cluster_v4(base + at(slot, g - peer * share, 0), r);
-          st_cluster_v4(base + at(slot, g - peer * share, 1), r + 4);
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k)
+            if (g0 + kGroups * k < end) {
+              st_cluster_v4(base + at(slot, g0 + kGroups * k - first, 0), r[k]);
+              st_cluster_v4(base + at(slot, g0 + kGroups * k - first, 1), r[k] + 4);
+            }
         }
       }
     }
     cluster_sync_all();
-    if (epi && ok) {
-      for (int g = rank * share; g < min(ng, (rank + 1) * share); ++g) {
+    if (group >= 0 && ok) {
+      const int first = rank * share;
+      for (int g = first + ((first ^ group) & 1); g < min(ng, first + share); g += kGroups) {
         uint32_t r[8];
         tmem_ld_16x256b_x1(tacc + 8 * g, r);
         tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * g, r + 4);
@@ -873,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int slot = 0; slot < p.splits - 1; ++slot)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float4 v = *reinterpret_cast<const float4*>(smem + at(slot, g - rank * share, h));
+            const float4 v = *reinterpret_cast<const float4*>(smem + at(slot, g - first, h));
             r[4 * h] = __float_as_uint(__uint_as_float(r[4 * h]) + v.x);
             r[4 * h + 1] = __float_as_uint(__uint_as_float(r[4 * h + 1]) + v.y);
             r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
@@ -948,6 +960,40 @@ cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int gr
               : launch<OutT, false, kWhole>(g, p, smem, grid, stream, why);
 }
 
+// Tile shapes and what a K tile of theirs takes, in us, when every SM has one:
+// from 48 .. 2000 tokens with 4096x7168, 7168x2048 and 2048x4096 weights.  A tile
+// of few tokens is bound by the loads of its weights, the large ones by what an
+// SM takes from L2 (64 bytes a clock), where a pair needs half the token bytes.
+struct Shape {
+  int tn, pair;
+  double k_tile_us;
+};
+constexpr Shape kShapes[] = {{32, 0, 0.18}, {64, 0, 0.205}, {128, 0, 0.28},
+                             {128, 1, 0.24}, {192, 1, 0.29}, {256, 1, 0.43}};
+
+// The shape with the shortest rounds of tiles.  How unevenly a routing fills the
+// experts is not known here: tiles are counted for 0.6 .. 1.5 times the mean.
+Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms) {
+  const double mean = static_cast<double>(g.rows) / busy;
+  Shape best = kShapes[0];
+  double best_us = 1e30;
+  for (const Shape& s : kShapes) {
+    const int features = (gate ? 64 : 128) * (s.pair ? 2 : 1);
+    double per_expert = 0;
+    if (g.offsets)
+      for (const double f : {0.6, 0.8, 1.0, 1.2, 1.5}) per_expert += std::ceil(f * mean / s.tn) / 5;
+    else
+      per_expert = std::ceil(mean / s.tn);
+    const double tiles = per_expert * busy * ((g.N + features - 1) / features);
+    const double us = std::ceil(tiles / (s.pair ? num_sms / 2 : num_sms)) * KT * s.k_tile_us;
+    if (us < best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why) {
@@ -967,13 +1013,11 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.status = g.status;
   p.inject = g.inject;
   p.vec = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
-  // Tokens per tile: the smallest that holds an average expert's rows with
-  // room for an uneven routing (an expert over the tile reads its weights twice).
+  const int KT = (g.K + kBK - 1) / kBK;
   const int busy = g.experts < g.rows ? g.experts : g.rows;
-  const int avg = (g.rows + busy - 1) / busy;
-  const int want = g.offsets ? avg + avg / 2 : avg;
-  p.tn = want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 192;
-  p.pair = p.tn == 192;
+  const Shape shape = choose_shape(g, gate, KT, busy, num_sms);
+  p.tn = shape.tn;
+  p.pair = shape.pair;
   const int features = (gate ? 64 : 128) * (p.pair ? 2 : 1);
   p.n_tiles = (g.N + features - 1) / features;
   const int x_rows = p.pair ? p.tn / 2 : p.tn;  // token rows in a CTA's shared memory
@@ -1000,10 +1044,17 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   // Tiles at most (whatever the offsets), and K splits where they leave SMs idle.
   const int64_t tiles = (static_cast<int64_t>(g.rows) / p.tn + busy) * p.n_tiles;
   const int64_t exact = g.offsets ? tiles : static_cast<int64_t>((g.rows + p.tn - 1) / p.tn) * p.n_tiles;
-  const int KT = (g.K + kBK - 1) / kBK;
+  // One tile takes 4.4 + 0.17 us per K tile on its SM; sharing K costs 2.5 us more
+  // for the exchange and divides the rest until HBM is the limit (some 65 SMs).
+  // Measured, one token: 7168x16384 17.9 -> 16.0 us with 2 CTAs, 2048x7168
+  // 9.2 -> 8.1 with 4, 1024x16384 15.2 -> 10.0 with 4 and 8.8 with 8 (clusters of 8
+  // find room for few at a time: 16 of them took 14.5 us).
   p.splits = 1;
-  if (!p.pair && p.tn <= 128)
-    while (p.splits < 8 && exact * p.splits * 2 <= num_sms && KT >= p.splits * 4) p.splits *= 2;
+  if (!p.pair)
+    p.splits = exact * 8 <= num_sms / 2 && KT >= 48 ? 8
+               : exact * 4 <= num_sms && KT >= 24   ? 4
+               : exact * 2 <= num_sms && KT >= 32   ? 2
+                                                    : 1;
   const int64_t workers = p.pair ? num_sms / 2 : num_sms;
   const int64_t grid = p.splits > 1 ? exact * p.splits : (exact < workers ? exact : workers) * (p.pair ? 2 : 1);
   const size_t smem = fixed + p.stages * stage;

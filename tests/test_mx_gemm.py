@@ -178,6 +178,47 @@ def test_nan_blocks_reach_only_their_rows_and_columns():
     np.testing.assert_array_equal(got[~bad], want[~bad])
 
 
+# Every tile shape (the launcher takes the one with the shortest rounds): 64, 128, 128, 192 and 256 tokens, the last
+# three on CTA pairs; whole tiles, ragged ends, and rows of C that are not 16-byte aligned.
+TILES = [(250, 4096, 64), (600, 3712, 64), (400, 4096, 96), (600, 4090, 160), (590, 4096, 320), (1000, 4096, 64),
+         (1013, 4093, 544)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", TILES)
+def test_every_tile_shape(dtype, m, n, k):
+    g = np.random.RandomState(m + n + k)
+    a, b = operand(m, k, g), operand(n, k, g)
+    x = mxref.decode(*a)
+    x1 = x @ mxref.decode(*b).T
+    ops = on_gpu(*a)
+    same(mx.gemm(*ops, *on_gpu(*b), out_dtype=dtype), x1)
+    # gated tiles have half as many features
+    n //= 2
+    low = 127 - int(np.log2(k) / 2) - 4
+    a = (a[0], g.randint(low, low + 3, (m, k // 32)).astype(np.uint8))
+    halves = [(t[:n], s[:n]) for t, s in (b, operand(n, k, g))]
+    x = mxref.decode(*a)
+    got = mx.dual_gemm(*on_gpu(*a), *on_gpu(*halves[0]), *on_gpu(*halves[1]), out_dtype=dtype)
+    gate_close(got, x @ mxref.decode(*halves[0]).T, x @ mxref.decode(*halves[1]).T)
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,tail", [([1000], 0), ([1000, 3, 250], 1), ([400], 7), ([130, 270, 0, 511], 0)])
+def test_every_tile_shape_with_experts(counts, tail):
+    n, k = 4096, 96
+    a, (b,), offsets, (want,) = grouped(counts, tail, n, k, 3)
+    same(mx.gemm(*a, *b, offsets=offsets), want)
+    n = 2048
+    a, (b1, b2), offsets, (x1, x2) = grouped(counts, tail, n, k, 4, both=True)
+    got = mx.dual_gemm(*a, *b1, *b2, offsets=offsets)
+    gate_close(got[:sum(counts)], x1[:sum(counts)], x2[:sum(counts)])
+    assert not f64(got[sum(counts):]).any()
+    assert _lib.device_status(True) == 0
+
+
 # ---------------------------------------------------------------- GPU: experts
 GROUPS = [([5], 0), ([0, 0, 0], 9), ([1, 0, 40, 0, 0, 3], 5), ([130, 1, 0, 127, 128, 129], 0), ([300, 0, 5], 20),
           ([2] * 64, 3), ([1000, 3, 250], 1), ([0] * 500 + [7] + [0] * 523, 2), ([33] * 12, 0), ([70, 65, 64, 100], 0)]

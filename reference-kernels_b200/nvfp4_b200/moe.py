@@ -26,7 +26,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib
+from . import _lib, mx
 from .inputs import FP4X2
 from .mx import _DTYPES, _byref, _device, _experts, _raw_stream, _require, E8M0, scale_blocks
 
@@ -162,3 +162,17 @@ def quantize_tokens(x: torch.Tensor, routing: Routing):
             x.data_ptr(), packed.data_ptr(), scales.data_ptr(), routing.offsets.data_ptr(), routing.slots.data_ptr(),
             _DTYPES[x.dtype], tokens, h, experts, top, 0, x.stride(0), 0, _raw_stream(dev)))))
     return packed, scales
+
+
+def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, down) -> torch.Tensor:
+    """The experts' MLP on x [T, H]: y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].
+
+    gate, up: operands (packed, scales) of [experts, N, H] weights, down of [experts, H, N], as mx.quantize makes them
+    (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  The tokens and the gated values are
+    quantised to MXFP4 on the way; x and the result are fp16, bf16 or fp32, and so are the values between the
+    products.  Six launches (seven for more than 4096 slots), no synchronisation."""
+    _require(gate[0].dim() == 3, f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
+    routing = sort(ids, gate[0].shape[0])
+    h = mx.dual_gemm(*quantize_tokens(x, routing), *gate, *up, offsets=routing.offsets, out_dtype=x.dtype)
+    y = mx.gemm(*mx.quantize(h, offsets=routing.offsets), *down, offsets=routing.offsets, out_dtype=x.dtype)
+    return combine(y, weights, routing)

@@ -28,7 +28,7 @@ import torch
 
 from . import _lib, mx
 from .inputs import FP4X2
-from .mx import _DTYPES, _byref, _device, _experts, _raw_stream, _require, E8M0, scale_blocks
+from .mx import _DTYPES, _byref, _device, _experts, _fail, _launch, _raw_stream, E8M0, scale_blocks
 
 
 class Routing(NamedTuple):
@@ -43,105 +43,118 @@ class Routing(NamedTuple):
 def sort(ids: torch.Tensor, experts: int) -> Routing:
     """Sorts the slots of ids [T, top] (int32 or int64, contiguous) by expert, stably; at most 1024 experts."""
     who = "moe.sort"
-    _require(ids.dtype in (torch.int32, torch.int64), f"{who}: ids must be int32 or int64, got {ids.dtype}")
-    _require(ids.dim() == 2 and ids.is_contiguous(), f"{who}: ids must be contiguous [tokens, top], "
-             f"got {tuple(ids.shape)} (strides {ids.stride()})")
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
+        _fail(f"{who}: ids must be int32 or int64, got {ids.dtype}")
+    shape = ids.shape
+    if len(shape) != 2 or not ids.is_contiguous():
+        _fail(f"{who}: ids must be contiguous [tokens, top], got {tuple(shape)} (strides {ids.stride()})")
     dev = _device(who, ids)
-    n = ids.numel()
+    n = shape[0] * shape[1]
     lib = _lib.load()
     need = lib.nvfp4_moe_sort_workspace(n, experts)
-    _require(need >= 0, f"{who}: experts={experts} must be 1 to 1024")
-    order = torch.empty((n,), dtype=torch.int32, device=ids.device)
-    slots = torch.empty(ids.shape, dtype=torch.int32, device=ids.device)
-    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=ids.device)
+    if need < 0:
+        _fail(f"{who}: experts={experts} must be 1 to 1024")
+    order = ids.new_empty((n,), dtype=torch.int32)
+    slots = ids.new_empty(shape, dtype=torch.int32)
+    offsets = ids.new_empty((experts + 1,), dtype=torch.int32)
     # On the caching allocator: a call on another stream, or a captured one, has its own.
-    work = torch.empty((need,), dtype=torch.uint8, device=ids.device) if need else None
-    _lib.check(lib.nvfp4_moe_sort(ids.data_ptr(), ids.element_size(), n, experts, order.data_ptr(), slots.data_ptr(),
-                                  offsets.data_ptr(), work.data_ptr() if need else None, need, _raw_stream(dev)))
+    work = ids.new_empty((need,), dtype=torch.uint8) if need else None
+    rc = lib.nvfp4_moe_sort(ids.data_ptr(), ids.element_size(), n, experts, order.data_ptr(), slots.data_ptr(),
+                            offsets.data_ptr(), work.data_ptr() if need else None, need, _raw_stream(dev))
+    if rc:
+        _lib.check(rc)
     return Routing(order, slots, offsets)
 
 
 def _check_routing(who: str, routing: Routing):
-    """(tokens, top, experts) of a routing."""
-    order, slots, offsets = routing
-    _require(slots.dtype == torch.int32 and slots.dim() == 2 and slots.is_contiguous(),
-             f"{who}: routing.slots must be contiguous int32 [tokens, top]")
-    return slots.shape[0], slots.shape[1], _experts(who, offsets)
+    """(slots, offsets, tokens, top, experts) of a routing."""
+    _, slots, offsets = routing
+    shape = slots.shape
+    if len(shape) != 2 or slots.dtype is not torch.int32 or not slots.is_contiguous():
+        _fail(f"{who}: routing.slots must be contiguous int32 [tokens, top]")
+    return slots, offsets, shape[0], shape[1], _experts(who, offsets)
 
 
-def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int, like: torch.Tensor | None = None) -> None:
-    _require(t.dtype in _DTYPES, f"{who}: {name} must be fp16, bf16 or fp32, got {t.dtype}")
-    _require(t.dim() == 2 and t.shape[0] == rows, f"{who}: {name} must be [{rows}, hidden], got {tuple(t.shape)}")
-    _require(t.stride(1) == 1 or t.shape[1] <= 1, f"{who}: {name} must have unit stride along the hidden dimension "
-             f"(strides {t.stride()})")
-    _require(like is None or (t.dtype == like.dtype and t.shape[1] == like.shape[1]),
-             f"{who}: {name} must have the other operand's type and hidden size")
+def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int):
+    """(dtype code, hidden, row stride) of t [rows, hidden]."""
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        _fail(f"{who}: {name} must be fp16, bf16 or fp32, got {t.dtype}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
+        _fail(f"{who}: {name} must be [{rows}, hidden], got {tuple(shape)}")
+    stride, unit = t.stride()
+    if unit != 1 and shape[1] > 1:
+        _fail(f"{who}: {name} must have unit stride along the hidden dimension (strides {t.stride()})")
+    return code, shape[1], stride
 
 
-def _check_weights(who: str, weights: torch.Tensor, routing: Routing) -> None:
-    _require(weights.dtype == torch.float32 and weights.shape == routing.slots.shape and weights.is_contiguous(),
-             f"{who}: weights must be contiguous fp32 {tuple(routing.slots.shape)}, "
-             f"got {weights.dtype} {tuple(weights.shape)} (strides {weights.stride()})")
+def _check_weights(who: str, weights: torch.Tensor, slots: torch.Tensor) -> None:
+    if weights.dtype is not torch.float32 or weights.shape != slots.shape or not weights.is_contiguous():
+        _fail(f"{who}: weights must be contiguous fp32 {tuple(slots.shape)}, "
+              f"got {weights.dtype} {tuple(weights.shape)} (strides {weights.stride()})")
+
+
+def _rows(name, x, grad, weights, out, dweights, slots, offsets, code, tokens, top, h, experts, stride, gstride, dev):
+    """One of the nvfp4_moe_* entry points that take nvfp4_moe_args."""
+    rc = getattr(_lib.load(), name)(_byref(_lib.MoeArgs(
+        x.data_ptr(), None if grad is None else grad.data_ptr(), None if weights is None else weights.data_ptr(),
+        out.data_ptr(), None if dweights is None else dweights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), code,
+        tokens, top, h, experts, 0, stride, gstride, _raw_stream(dev))))
+    if rc:
+        _lib.check(rc)
 
 
 def gather(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """x [T, H] -> xs [T*top, H], each token's row at each of its sorted rows."""
     who = "moe.gather"
-    tokens, top, experts = _check_routing(who, routing)
-    _check_matrix(who, "x", x, tokens)
-    dev = _device(who, x, routing.slots, routing.offsets)
-    h = x.shape[1]
-    xs = torch.empty((tokens * top, h), dtype=x.dtype, device=x.device)
-    _lib.check(_lib.load().nvfp4_moe_gather(_byref(_lib.MoeArgs(
-        x.data_ptr(), None, None, xs.data_ptr(), None, routing.slots.data_ptr(), routing.offsets.data_ptr(),
-        _DTYPES[x.dtype], tokens, top, h, experts, 0, x.stride(0), 0, _raw_stream(dev)))))
+    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    code, h, stride = _check_matrix(who, "x", x, tokens)
+    dev = _device(who, x, slots, offsets)
+    xs = x.new_empty((tokens * top, h))
+    _rows("nvfp4_moe_gather", x, None, None, xs, None, slots, offsets, code, tokens, top, h, experts, stride, 0, dev)
     return xs
 
 
 def gather_backward(dxs: torch.Tensor, routing: Routing) -> torch.Tensor:
     """The gradient of gather: dxs [T*top, H] -> dx [T, H], the sum over each token's rows."""
     who = "moe.gather_backward"
-    tokens, top, experts = _check_routing(who, routing)
-    _check_matrix(who, "dxs", dxs, tokens * top)
-    dev = _device(who, dxs, routing.slots)
-    h = dxs.shape[1]
-    dx = torch.empty((tokens, h), dtype=dxs.dtype, device=dxs.device)
-    _lib.check(_lib.load().nvfp4_moe_gather_backward(_byref(_lib.MoeArgs(
-        dxs.data_ptr(), None, None, dx.data_ptr(), None, routing.slots.data_ptr(), None,
-        _DTYPES[dxs.dtype], tokens, top, h, experts, 0, dxs.stride(0), 0, _raw_stream(dev)))))
+    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    code, h, stride = _check_matrix(who, "dxs", dxs, tokens * top)
+    dev = _device(who, dxs, slots, offsets)
+    dx = dxs.new_empty((tokens, h))
+    _rows("nvfp4_moe_gather_backward", dxs, None, None, dx, None, slots, offsets, code, tokens, top, h, experts,
+          stride, 0, dev)
     return dx
 
 
 def combine(ys: torch.Tensor, weights: torch.Tensor, routing: Routing) -> torch.Tensor:
     """ys [T*top, H], weights fp32 [T, top] -> y [T, H], the weighted sum of each token's rows (no row: zeros)."""
     who = "moe.combine"
-    tokens, top, experts = _check_routing(who, routing)
-    _check_matrix(who, "ys", ys, tokens * top)
-    _check_weights(who, weights, routing)
-    dev = _device(who, ys, weights, routing.slots)
-    h = ys.shape[1]
-    y = torch.empty((tokens, h), dtype=ys.dtype, device=ys.device)
-    _lib.check(_lib.load().nvfp4_moe_combine(_byref(_lib.MoeArgs(
-        ys.data_ptr(), None, weights.data_ptr(), y.data_ptr(), None, routing.slots.data_ptr(), None,
-        _DTYPES[ys.dtype], tokens, top, h, experts, 0, ys.stride(0), 0, _raw_stream(dev)))))
+    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    code, h, stride = _check_matrix(who, "ys", ys, tokens * top)
+    _check_weights(who, weights, slots)
+    dev = _device(who, ys, weights, slots, offsets)
+    y = ys.new_empty((tokens, h))
+    _rows("nvfp4_moe_combine", ys, None, weights, y, None, slots, offsets, code, tokens, top, h, experts, stride, 0,
+          dev)
     return y
 
 
 def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, routing: Routing):
     """The gradients of combine: (dys [T*top, H], dweights fp32 [T, top])."""
     who = "moe.combine_backward"
-    tokens, top, experts = _check_routing(who, routing)
-    _check_matrix(who, "dy", dy, tokens)
-    _check_matrix(who, "ys", ys, tokens * top, dy)
-    _check_weights(who, weights, routing)
-    dev = _device(who, dy, ys, weights, routing.slots, routing.offsets)
-    h = dy.shape[1]
-    dys = torch.empty((tokens * top, h), dtype=ys.dtype, device=ys.device)
-    dweights = torch.empty((tokens, top), dtype=torch.float32, device=ys.device)
-    _lib.check(_lib.load().nvfp4_moe_combine_backward(_byref(_lib.MoeArgs(
-        ys.data_ptr(), dy.data_ptr(), weights.data_ptr(), dys.data_ptr(), dweights.data_ptr(),
-        routing.slots.data_ptr(), routing.offsets.data_ptr(), _DTYPES[ys.dtype], tokens, top, h, experts, 0,
-        ys.stride(0), dy.stride(0), _raw_stream(dev)))))
+    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    code, h, gstride = _check_matrix(who, "dy", dy, tokens)
+    ycode, yh, stride = _check_matrix(who, "ys", ys, tokens * top)
+    if ycode != code or yh != h:
+        _fail(f"{who}: ys must have dy's type and hidden size")
+    _check_weights(who, weights, slots)
+    dev = _device(who, dy, ys, weights, slots, offsets)
+    dys = ys.new_empty((tokens * top, h))
+    dweights = weights.new_empty((tokens, top))
+    _rows("nvfp4_moe_combine_backward", ys, dy, weights, dys, dweights, slots, offsets, code, tokens, top, h, experts,
+          stride, gstride, dev)
     return dys, dweights
 
 
@@ -149,18 +162,17 @@ def quantize_tokens(x: torch.Tensor, routing: Routing):
     """x [T, H] (fp16, bf16 or fp32, H % 32 == 0) -> the MXFP4 operand (packed [T*top, H/2], scales) of its sorted
     rows: mx.quantize of gather(x), with each token quantised once.  Rows behind the last expert's are not written."""
     who = "moe.quantize_tokens"
-    tokens, top, experts = _check_routing(who, routing)
-    _check_matrix(who, "x", x, tokens)
-    h = x.shape[1]
-    _require(h > 0 and h % 32 == 0, f"{who}: hidden={h} must be a positive multiple of 32")
-    dev = _device(who, x, routing.slots, routing.offsets)
+    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    code, h, stride = _check_matrix(who, "x", x, tokens)
+    if h == 0 or h % 32:
+        _fail(f"{who}: hidden={h} must be a positive multiple of 32")
+    dev = _device(who, x, slots, offsets)
     rows = tokens * top
-    packed = torch.empty((rows, h // 2), dtype=FP4X2, device=x.device)
-    scales = torch.empty((scale_blocks(rows, experts), -(-h // 128), 32, 4, 4), dtype=E8M0, device=x.device)
+    packed = x.new_empty((rows, h // 2), dtype=FP4X2)
+    scales = x.new_empty((scale_blocks(rows, experts), -(-h // 128), 32, 4, 4), dtype=E8M0)
     if rows:
-        _lib.check(_lib.load().nvfp4_mx_quantize(_byref(_lib.MxQuantArgs(
-            x.data_ptr(), packed.data_ptr(), scales.data_ptr(), routing.offsets.data_ptr(), routing.slots.data_ptr(),
-            _DTYPES[x.dtype], tokens, h, experts, top, 0, x.stride(0), 0, _raw_stream(dev)))))
+        _launch("nvfp4_mx_quantize", x, packed, scales, offsets, slots, code, tokens, h, experts, top, 0, stride, 0,
+                dev)
     return packed, scales
 
 
@@ -171,7 +183,8 @@ def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, dow
     (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  The tokens and the gated values are
     quantised to MXFP4 on the way; x and the result are fp16, bf16 or fp32, and so are the values between the
     products.  Six launches (seven for more than 4096 slots), no synchronisation."""
-    _require(gate[0].dim() == 3, f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
+    if gate[0].dim() != 3:
+        _fail(f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
     routing = sort(ids, gate[0].shape[0])
     h = mx.dual_gemm(*quantize_tokens(x, routing), *gate, *up, offsets=routing.offsets, out_dtype=x.dtype)
     y = mx.gemm(*mx.quantize(h, offsets=routing.offsets), *down, offsets=routing.offsets, out_dtype=x.dtype)

@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 from .inputs import FP4X2
-from .ops import _post
+from .ops import _CHECK_STATUS, _post
 
 E8M0 = torch.float8_e8m0fnu
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -38,28 +38,30 @@ _current_device = torch._C._cuda_getDevice
 _byref = ctypes.byref
 
 
-def _require(cond: bool, msg: str) -> None:
-    if not cond:
-        raise _lib.Nvfp4Error(msg)
+def _fail(msg: str):
+    """Calls of a few microseconds of GPU time are paced by the host: checks here test first and format their
+    message (which takes longer than the test) only when they fail."""
+    raise _lib.Nvfp4Error(msg)
 
 
 def _device(who: str, t: torch.Tensor, *others) -> int:
     """The device of every tensor (None: not given), which has to be the current one."""
     dev = t.get_device()
-    _require(dev >= 0, f"{who}: expected a CUDA tensor (no CPU fallback)")
+    if dev < 0:
+        _fail(f"{who}: expected a CUDA tensor (no CPU fallback)")
     for o in others:
         if o is not None and o.get_device() != dev:
-            _require(False, f"{who}: tensors on different devices (cuda:{dev} and {o.device})")
-    _require(dev == _current_device(),
-             f"{who}: the tensors are on cuda:{dev} but cuda:{_current_device()} is current; "
-             f"call inside torch.cuda.device({dev})")
+            _fail(f"{who}: tensors on different devices (cuda:{dev} and {o.device})")
+    if dev != _current_device():
+        _fail(f"{who}: the tensors are on cuda:{dev} but cuda:{_current_device()} is current; "
+              f"call inside torch.cuda.device({dev})")
     return dev
 
 
 def _experts(who: str, offsets: torch.Tensor) -> int:
-    _require(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous()
-             and 2 <= offsets.shape[0] <= 1025,
-             f"{who}: offsets must be a contiguous int32 [experts + 1], at most 1024 experts")
+    if not (offsets.dtype is torch.int32 and offsets.dim() == 1 and 2 <= offsets.shape[0] <= 1025
+            and offsets.is_contiguous()):
+        _fail(f"{who}: offsets must be a contiguous int32 [experts + 1], at most 1024 experts")
     return offsets.shape[0] - 1
 
 
@@ -69,19 +71,21 @@ def scale_blocks(rows: int, experts: int | None = None) -> int:
 
 
 def _check_operand(who: str, packed: torch.Tensor, scales: torch.Tensor, dim: int, experts: int | None = None):
-    """(matrices, rows, K) of an operand; ``dim``: of packed; ``experts``: rows are sorted by expert."""
-    _require(packed.element_size() == 1 and packed.dim() == dim and packed.is_contiguous(),
-             f"{who}: codes must be contiguous float4_e2m1fn_x2 or uint8 of {dim} dimensions, "
-             f"got {packed.dtype} {tuple(packed.shape)} (strides {packed.stride()})")
-    rows, k = packed.shape[-2], 2 * packed.shape[-1]
-    _require(k > 0 and k % 32 == 0, f"{who}: K={k} must be a positive multiple of 32")
-    want = (scale_blocks(rows, experts), -(-k // 128), 32, 4, 4)
+    """The shape of an operand's packed tensor; ``dim``: its dimensions; ``experts``: rows are sorted by expert."""
+    shape = packed.shape
+    if len(shape) != dim or packed.element_size() != 1 or not packed.is_contiguous():
+        _fail(f"{who}: codes must be contiguous float4_e2m1fn_x2 or uint8 of {dim} dimensions, "
+              f"got {packed.dtype} {tuple(shape)} (strides {packed.stride()})")
+    k2 = shape[-1]
+    if k2 == 0 or k2 % 16:
+        _fail(f"{who}: K={2 * k2} must be a positive multiple of 32")
+    want = (scale_blocks(shape[-2], experts), -(-k2 // 64), 32, 4, 4)
     if dim == 3:
-        want = (packed.shape[0], *want)
-    _require(scales.element_size() == 1 and tuple(scales.shape) == want and scales.is_contiguous(),
-             f"{who}: scales must be contiguous float8_e8m0fnu or uint8 {want}, "
-             f"got {scales.dtype} {tuple(scales.shape)} (strides {scales.stride()})")
-    return (packed.shape[0] if dim == 3 else 1), rows, k
+        want = (shape[0], *want)
+    if scales.shape != want or scales.element_size() != 1 or not scales.is_contiguous():
+        _fail(f"{who}: scales must be contiguous float8_e8m0fnu or uint8 {want}, "
+              f"got {scales.dtype} {tuple(scales.shape)} (strides {scales.stride()})")
+    return shape
 
 
 def quantize(x: torch.Tensor, axis: int = -1, offsets: torch.Tensor | None = None):
@@ -100,35 +104,60 @@ def quantize(x: torch.Tensor, axis: int = -1, offsets: torch.Tensor | None = Non
     offsets: the rows are sorted by expert.  Codes of rows behind the last
     expert's are not written."""
     who = "mx.quantize"
-    _require(x.dtype in _DTYPES, f"{who}: x must be fp16, bf16 or fp32, got {x.dtype}")
-    _require(x.dim() in (2, 3), f"{who}: x must be [rows, K] or [experts, rows, K], got {tuple(x.shape)}")
-    rows, k = x.shape[-2:]
-    columns = x.dim() == 2 and axis == 0
-    _require(columns or axis in (-1, x.dim() - 1), f"{who}: axis={axis} must be the last, or 0 of a matrix")
-    _require(k > 0 and (columns or k % 32 == 0), f"{who}: K={k} must be a positive multiple of 32")
-    _require(x.stride(-1) == 1 or k == 1, f"{who}: x must have unit stride along K (strides {x.stride()})")
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        _fail(f"{who}: x must be fp16, bf16 or fp32, got {x.dtype}")
+    shape, strides = x.shape, x.stride()
+    dim = len(shape)
+    if dim != 2 and dim != 3:
+        _fail(f"{who}: x must be [rows, K] or [experts, rows, K], got {tuple(shape)}")
+    rows, k = shape[-2], shape[-1]
+    columns = axis == 0 and dim == 2
+    if not columns and axis != -1 and axis != dim - 1:
+        _fail(f"{who}: axis={axis} must be the last, or 0 of a matrix")
+    if k == 0 or (k % 32 and not columns):
+        _fail(f"{who}: K={k} must be a positive multiple of 32")
+    if strides[-1] != 1 and k != 1:
+        _fail(f"{who}: x must have unit stride along K (strides {strides})")
     dev = _device(who, x, offsets)
-    experts = x.shape[0] if x.dim() == 3 else 1
     if columns:
-        _require(offsets is None, f"{who}: axis=0 takes no offsets")
+        if offsets is not None:
+            _fail(f"{who}: axis=0 takes no offsets")
         kt = -(-rows // 32) * 32
-        packed = torch.empty((k, kt // 2), dtype=FP4X2, device=x.device)
-        scales = torch.empty((-(-k // 128), -(-kt // 128), 32, 4, 4), dtype=E8M0, device=x.device)
-    elif offsets is not None:
-        _require(x.dim() == 2, f"{who}: offsets need x [rows, K]")
+        packed = x.new_empty((k, kt // 2), dtype=FP4X2)
+        scales = x.new_empty((-(-k // 128), -(-kt // 128), 32, 4, 4), dtype=E8M0)
+        if rows:
+            _launch("nvfp4_mx_quantize", x, packed, scales, None, None, code, rows, k, 1, 0, 1, strides[0], 0, dev)
+        return packed, scales
+    experts = None
+    if offsets is not None:
+        if dim != 2:
+            _fail(f"{who}: offsets need x [rows, K]")
         experts = _experts(who, offsets)
-        packed = torch.empty((rows, k // 2), dtype=FP4X2, device=x.device)
-        scales = torch.empty((scale_blocks(rows, experts), -(-k // 128), 32, 4, 4), dtype=E8M0, device=x.device)
+    blocks = (scale_blocks(rows, experts), -(-k // 128), 32, 4, 4)
+    if dim == 2:
+        packed = x.new_empty((rows, k // 2), dtype=FP4X2)
+        scales = x.new_empty(blocks, dtype=E8M0)
+        if rows:
+            _launch("nvfp4_mx_quantize", x, packed, scales, offsets, None, code, rows, k, experts or 1, 0, 0,
+                    strides[0], 0, dev)
     else:
-        packed = torch.empty((*x.shape[:-1], k // 2), dtype=FP4X2, device=x.device)
-        scales = torch.empty((*x.shape[:-2], -(-rows // 128), -(-k // 128), 32, 4, 4), dtype=E8M0, device=x.device)
-    if packed.numel():
-        args = _lib.MxQuantArgs(x.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                None if offsets is None else offsets.data_ptr(), None, _DTYPES[x.dtype], rows, k,
-                                experts, 0, columns, x.stride(-2), x.stride(0) if x.dim() == 3 else 0,
-                                _raw_stream(dev))
-        _lib.check(_lib.load().nvfp4_mx_quantize(_byref(args)))
+        packed = x.new_empty((shape[0], rows, k // 2), dtype=FP4X2)
+        scales = x.new_empty((shape[0], *blocks), dtype=E8M0)
+        if rows and shape[0]:
+            _launch("nvfp4_mx_quantize", x, packed, scales, None, None, code, rows, k, shape[0], 0, 0, strides[1],
+                    strides[0], dev)
     return packed, scales
+
+
+def _launch(name, x, packed, scales, offsets, slots, dtype, rows, k, experts, top, columns, rstride, estride, dev):
+    """nvfp4_mx_quantize or nvfp4_mx_dequantize."""
+    rc = getattr(_lib.load(), name)(_byref(_lib.MxQuantArgs(
+        x.data_ptr(), packed.data_ptr(), scales.data_ptr(), None if offsets is None else offsets.data_ptr(),
+        None if slots is None else slots.data_ptr(), dtype, rows, k, experts, top, columns, rstride, estride,
+        _raw_stream(dev))))
+    if rc:
+        _lib.check(rc)
 
 
 def dequantize(packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -136,42 +165,50 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor
     """The values of an operand, [rows, K] or [E, rows, K] of ``dtype`` (exact in bf16 and fp32; fp16 rounds, and
     overflows above 65504).  With offsets, rows behind the last expert's are zeros."""
     who = "mx.dequantize"
-    _require(dtype in _DTYPES, f"{who}: dtype must be fp16, bf16 or fp32, got {dtype}")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        _fail(f"{who}: dtype must be fp16, bf16 or fp32, got {dtype}")
     experts = None if offsets is None else _experts(who, offsets)
-    matrices, rows, k = _check_operand(who, packed, scales, 2 if offsets is not None or packed.dim() != 3 else 3,
-                                       experts)
+    shape = _check_operand(who, packed, scales, 3 if experts is None and packed.dim() == 3 else 2, experts)
     dev = _device(who, packed, scales, offsets)
-    out = torch.empty((*packed.shape[:-1], k), dtype=dtype, device=packed.device)
+    rows, k = shape[-2], 2 * shape[-1]
+    out = packed.new_empty((*shape[:-1], k), dtype=dtype)
     if out.numel():
-        args = _lib.MxQuantArgs(out.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                None if offsets is None else offsets.data_ptr(), None, _DTYPES[dtype], rows, k,
-                                matrices if experts is None else experts, 0, 0, k, rows * k, _raw_stream(dev))
-        _lib.check(_lib.load().nvfp4_mx_dequantize(_byref(args)))
+        if experts is None:
+            experts = shape[0] if len(shape) == 3 else 1
+        _launch("nvfp4_mx_dequantize", out, packed, scales, offsets, None, code, rows, k, experts, 0, 0, k, rows * k,
+                dev)
     return out
 
 
 def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype):
-    _require(out_dtype in _DTYPES, f"{who}: out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
-    experts = None
+    code = _DTYPES.get(out_dtype)
+    if code is None:
+        _fail(f"{who}: out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
+    experts, dim = None, 2
     if offsets is not None:
-        experts = _experts(who, offsets)
-        _require(b1.dim() == 3 and b1.shape[0] == experts,
-                 f"{who}: offsets of {experts} experts need weights [{experts}, N, K/2], got {tuple(b1.shape)}")
-    _, rows, k = _check_operand(who, a, sa, 2, experts)
-    for b, s in ((b1, s1), (b2, s2)):
-        if b is not None:
-            _, n, kb = _check_operand(who, b, s, 2 if experts is None else 3)
-            _require(kb == k and b.shape == b1.shape, f"{who}: weights {tuple(b.shape)} do not fit tokens with K={k}"
-                     + ("" if b is b1 else f" and weights {tuple(b1.shape)}"))
+        experts, dim = _experts(who, offsets), 3
+        if b1.dim() != 3 or b1.shape[0] != experts:
+            _fail(f"{who}: offsets of {experts} experts need weights [{experts}, N, K/2], got {tuple(b1.shape)}")
+    rows, k2 = _check_operand(who, a, sa, 2, experts)
+    shape = _check_operand(who, b1, s1, dim)
+    if shape[-1] != k2:
+        _fail(f"{who}: weights {tuple(shape)} do not fit tokens with K={2 * k2}")
+    if b2 is not None and _check_operand(who, b2, s2, dim) != shape:
+        _fail(f"{who}: weights {tuple(b2.shape)} do not fit weights {tuple(shape)}")
     dev = _device(who, a, sa, b1, s1, b2, s2, offsets)
-    c = torch.empty((rows, n), dtype=out_dtype, device=a.device)
-    if c.numel():
-        args = _lib.MxGemmArgs(a.data_ptr(), b1.data_ptr(), None if b2 is None else b2.data_ptr(), sa.data_ptr(),
-                               s1.data_ptr(), None if b2 is None else s2.data_ptr(), c.data_ptr(),
-                               None if offsets is None else offsets.data_ptr(), rows, n, k, experts or 1,
-                               _DTYPES[out_dtype], 0, n, _raw_stream(dev))
-        _lib.check(_lib.load().nvfp4_mx_gemm(_byref(args)))
-        _post()
+    n = shape[-2]
+    c = a.new_empty((rows, n), dtype=out_dtype)
+    if rows and n:
+        gated = b2 is not None
+        rc = _lib.load().nvfp4_mx_gemm(_byref(_lib.MxGemmArgs(
+            a.data_ptr(), b1.data_ptr(), b2.data_ptr() if gated else None, sa.data_ptr(), s1.data_ptr(),
+            s2.data_ptr() if gated else None, c.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, n,
+            2 * k2, experts or 1, code, 0, n, _raw_stream(dev))))
+        if rc:
+            _lib.check(rc)
+        if _CHECK_STATUS:
+            _post()
     return c
 
 

@@ -220,7 +220,7 @@ int nvfp4_dual_gemm_call(const nvfp4_gemm_args* args);
  * Per block of 32: code = max(floor(log2(amax)) - 2 + 127, 0), values
  * e2m1_rn_satfinite(x * 2^(127 - code)); code 255 and zero values where the
  * block holds a NaN or an infinity.
- * nvfp4_mx_dequantize writes values of type dtype to x (contiguous, 16-byte aligned). */
+ * nvfp4_mx_dequantize writes values of type dtype to x (contiguous, 32-byte aligned). */
 typedef struct {
   const void* x;
   void* packed;

@@ -436,16 +436,16 @@ static int mx_quant_args(const char* name, const nvfp4_mx_quant_args* x, bool qu
   if (x->slots && (!quantize || !x->offsets || x->top < 0))
     return fail(NVFP4_ERR_SHAPE, "%s: slots need offsets and top >= 0", name);
   const int64_t rows = x->offsets ? x->rows : static_cast<int64_t>(x->rows) * x->experts;
-  const int64_t units = rows * ((static_cast<int64_t>(x->K) + 511) / 512);
+  const int64_t units = rows * ((static_cast<int64_t>(x->K) + 127) / 128 * 4);  // scales, padding included
   const int64_t sorted = x->slots ? static_cast<int64_t>(x->rows) * x->top : rows;
   if (rows > INT32_MAX || units > INT32_MAX || sorted > INT32_MAX || (x->columns && x->rows > 65535 * 256))
     return fail(NVFP4_ERR_SHAPE, "%s: too many rows", name);
   if (rows > 0 && sorted > 0) {
     if (!x->x || !x->packed || !x->scales) return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
-    if (!aligned(x->x, quantize ? dtype_size(x->dtype) : 16) || !aligned(x->packed, 16) || !aligned(x->scales, 16) ||
+    if (!aligned(x->x, quantize ? dtype_size(x->dtype) : 32) || !aligned(x->packed, 16) || !aligned(x->scales, 16) ||
         !aligned(x->offsets, 4) || !aligned(x->slots, 4))
       return fail(NVFP4_ERR_ALIGN, "%s: codes and scales need 16-byte alignment, x that of its type%s", name,
-                  quantize ? "" : " and 16 bytes");
+                  quantize ? "" : " and 32 bytes");
   }
   a = MxQuantArgs{x->x,       x->packed, x->scales, x->offsets, x->slots, x->dtype, static_cast<int>(rows), x->K, x->rows,
                   x->experts, x->top,    static_cast<int>(sorted), x->columns, x->x_rstride, x->x_estride};

@@ -28,14 +28,22 @@ namespace {
 
 // ------------------------------------------------------------------ sort
 // A stable counting sort.  A CTA takes a run of slots and each of its 32 warps
-// a part of that run; within a warp 32 slots at a time are ranked with
-// match_any.  hist[warp][expert] in shared memory first counts, then (after
+// a part of that run; within a warp 32 slots at a time are ranked by ballots.  hist[warp][expert] in shared memory first counts, then (after
 // sums over the warps, the CTAs and the experts) holds the next free row.
-// One CTA does short lists in one launch; longer ones take a second launch,
-// before it, that counts each CTA's run (counts[cta][expert]), and each CTA
-// adds up the counts of the CTAs before it itself.
+// One CTA does short lists, a cluster of eight longer ones, whose CTAs read one
+// another's counts from distributed shared memory.  Lists that keep a cluster's
+// warps busy for long take a second launch, before it, that counts each CTA's run
+// to memory (counts[cta][expert]), and a CTA per SM at most.
 constexpr int kSortWarps = 32;
 constexpr int kSortThreads = 32 * kSortWarps;
+
+constexpr int kSortCluster = 8;
+
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 template <typename Id>
 __device__ __forceinline__ int expert_id(const Id* ids, int slot, int E) {
@@ -43,20 +51,47 @@ __device__ __forceinline__ int expert_id(const Id* ids, int slot, int E) {
   return v >= 0 && v < E ? static_cast<int>(v) : -1;
 }
 
+// The lanes that hold the same id (-1 .. E - 1): one ballot per bit.  (A
+// match.any took about 1 us for a step of 32 warps.)
+__device__ __forceinline__ uint32_t same_id(int id, int E) {
+  uint32_t peers = 0xffffffffu;
+  for (int bit = 1; bit <= E; bit <<= 1) {  // -1 counts as E
+    const bool set = (id < 0 ? E : id) & bit;
+    const uint32_t with = __ballot_sync(0xffffffffu, set);
+    peers &= set ? with : ~with;
+  }
+  return peers;
+}
+
+// Calls f(slot, id) for this warp's part of the run [begin, end), 32 slots at a
+// time (id -1: not routed, or behind the end), with the loads of four such steps
+// in flight together.
+template <typename Id, typename F>
+__device__ __forceinline__ void for_run(const Id* ids, int begin, int end, int E, F f) {
+  constexpr int kAhead = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = ((end - begin + kSortThreads - 1) / kSortThreads) * 32;  // slots per warp
+  const int b = begin + warp * per, e = min(b + per, end);
+  for (int s0 = b; s0 < e; s0 += 32 * kAhead) {
+    int id[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int slot = s0 + 32 * k + lane;
+      id[k] = slot < e ? expert_id(ids, slot, E) : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (s0 + 32 * k < e) f(s0 + 32 * k + lane, id[k], e);
+  }
+}
+
 // Counts the run [begin, end) into hist[warp][E].
 template <typename Id>
 __device__ __forceinline__ void count_run(const Id* ids, int begin, int end, int E, int* hist) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* mine = hist + warp * E;
-  const int per = ((end - begin + kSortThreads - 1) / kSortThreads) * 32;  // slots per warp
-  const int b = begin + warp * per, e = min(b + per, end);
-  for (int s0 = b; s0 < e; s0 += 32) {
-    const int slot = s0 + lane;
-    const int id = slot < e ? expert_id(ids, slot, E) : -1;
-    const uint32_t peers = __match_any_sync(0xffffffffu, id);
-    if (id >= 0 && (peers & ((1u << lane) - 1)) == 0) mine[id] += __popc(peers);
-    __syncwarp();
-  }
+  int* mine = hist + (threadIdx.x >> 5) * E;
+  for_run(ids, begin, end, E, [&](int, int id, int) {
+    if (id >= 0) atomicAdd(mine + id, 1);  // counts alone: their order does not matter
+  });
 }
 
 template <typename Id>
@@ -77,9 +112,10 @@ __global__ void __launch_bounds__(kSortThreads) moe_count_kernel(const MoeSortAr
   }
 }
 
-template <typename Id>
+template <typename Id, bool kCluster>
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const MoeSortArgs a) {
   extern __shared__ int hist[];
+  __shared__ int cta_count[kCluster ? kMaxExperts : 1];
   __shared__ int warp_sum[kSortWarps];
   __shared__ int routed;
   if (threadIdx.x == 0) pdl_allow_dependents();
@@ -94,7 +130,23 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const MoeSortArg
   // Thread e: expert e's total, and its slots in the CTAs before this one.
   const int e = threadIdx.x;
   int total = 0, before = 0;
-  if (e < E) {
+  if (kCluster) {
+    int mine = 0;
+    if (e < E) {
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) mine += hist[w * E + e];
+      cta_count[e] = mine;
+    }
+    cluster_sync_all();
+    if (e < E) {
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) {
+        const int n = ld_cluster(map_peer(smem_u32(&cta_count[e]), c));
+        total += n;
+        before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+    }
+  } else if (e < E) {
     if (gridDim.x == 1) {
 #pragma unroll 8
       for (int w = 0; w < kSortWarps; ++w) total += hist[w * E + e];
@@ -142,12 +194,8 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const MoeSortArg
   }
   __syncthreads();
   int* mine = hist + warp * E;
-  const int per = ((end - begin + kSortThreads - 1) / kSortThreads) * 32;
-  const int b = begin + warp * per, stop = min(b + per, end);
-  for (int s0 = b; s0 < stop; s0 += 32) {
-    const int slot = s0 + lane;
-    const int id = slot < stop ? expert_id(ids, slot, E) : -1;
-    const uint32_t peers = __match_any_sync(0xffffffffu, id);
+  for_run(ids, begin, end, E, [&](int slot, int id, int stop) {
+    const uint32_t peers = same_id(id, E);
     const int rank = __popc(peers & ((1u << lane) - 1));
     int row = -1;
     if (id >= 0) row = mine[id] + rank;
@@ -156,29 +204,64 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const MoeSortArg
     __syncwarp();
     if (slot < stop) a.slots[slot] = row;
     if (row >= 0) a.order[row] = slot;
-  }
+  });
+  if (kCluster) cluster_sync_all();  // the others have read this CTA's counts
   // Rows that no slot has.
   for (int i = routed + blockIdx.x * kSortThreads + threadIdx.x; i < a.slots_n; i += gridDim.x * kSortThreads)
     a.order[i] = -1;
 }
 
 // ------------------------------------------------------------------ rows
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ void put(__half& d, float v) { d = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(float& d, float v) { d = v; }
-
-// N elements that are loaded and stored together: 16 bytes where rows and
-// bases allow it, else as many as divide the row and its address.
+// N elements that are loaded and stored together: 16 bytes where rows and bases
+// allow it, else as many as divide the row and its address.  Held as whole
+// words: as an array of 16-bit values the compiler gave each a register.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-  T v[N];
+struct Pack {
+  static constexpr int kBytes = sizeof(T) * N;
+  using Word = std::conditional_t<kBytes == 2, uint16_t, uint32_t>;
+  struct alignas(kBytes) Raw {
+    Word w[kBytes / sizeof(Word)];
+  } raw;
+
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(raw.w[i]);
+    } else {
+      const uint32_t half = kBytes == 2 ? raw.w[0] : (i & 1 ? raw.w[i / 2] >> 16 : raw.w[i / 2] & 0xffffu);
+      if constexpr (std::is_same<T, __half>::value)
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
+      else
+        return __uint_as_float(half << 16);
+    }
+  }
+  // All N at once, from fp32.
+  __device__ __forceinline__ void set(const float (&v)[N]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw.w[i] = __float_as_uint(v[i]);
+    } else if constexpr (N == 1) {
+      raw.w[0] = bits(v[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) raw.w[i] = bits(v[2 * i]) | bits(v[2 * i + 1]) << 16;
+    }
+  }
+
+ private:
+  static __device__ __forceinline__ uint32_t bits(float v) {
+    if constexpr (std::is_same<T, __half>::value)
+      return __half_as_ushort(__float2half_rn(v));
+    else
+      return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  }
 };
 
 constexpr int kRowThreads = 128;
-constexpr int kUnroll = 4;  // packs per thread and step: loads in flight
+// Packs per thread and step: `bytes` of loads in flight.
+template <typename T, int N>
+__host__ __device__ constexpr int in_flight(int bytes) {
+  return bytes / static_cast<int>(sizeof(T) * N) < 16 ? bytes / static_cast<int>(sizeof(T) * N) : 16;
+}
 
 // Zeroes the rows of out [rows][H] that no slot has (from offsets[E] on).
 template <typename T, int N>
@@ -186,51 +269,54 @@ __device__ __forceinline__ void zero_tail(T* out, const int* offsets, int E, int
   const int first = min(max(offsets[E], 0), rows);
   const int64_t n = static_cast<int64_t>(rows - first) * packs;
   Pack<T, N> z;
-#pragma unroll
-  for (int i = 0; i < N; ++i) put(z.v[i], 0.f);
+  const float zeros[N] = {};
+  z.set(zeros);
   Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(first) * packs;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x)
     dst[i] = z;
 }
 
-// A unit is one token and kRowThreads * kUnroll packs of its row.
+// A unit is one token and kRowThreads * kU packs of its row.
 template <typename T, int N>
 __global__ void __launch_bounds__(kRowThreads) moe_gather_kernel(const MoeRowArgs a) {
   if (threadIdx.x == 0) pdl_allow_dependents();
   pdl_wait();
+  constexpr int kU = in_flight<T, N>(64);
   const int packs = a.hidden / N;
-  const int per_row = (packs + kRowThreads * kUnroll - 1) / (kRowThreads * kUnroll);
+  const int per_row = (packs + kRowThreads * kU - 1) / (kRowThreads * kU);
   const int64_t units = static_cast<int64_t>(a.tokens) * per_row;
   const int rows = a.tokens * a.top;
   T* const out = static_cast<T*>(a.out);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int t = static_cast<int>(u / per_row);
-    const int p0 = static_cast<int>(u - static_cast<int64_t>(t) * per_row) * kRowThreads * kUnroll + threadIdx.x;
+    const int p0 = static_cast<int>(u - static_cast<int64_t>(t) * per_row) * kRowThreads * kU + threadIdx.x;
     const Pack<T, N>* src =
         reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.in) + static_cast<int64_t>(t) * a.in_stride);
-    Pack<T, N> v[kUnroll];
+    Pack<T, N> v[kU];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i)
+    for (int i = 0; i < kU; ++i)
       if (p0 + i * kRowThreads < packs) v[i] = src[p0 + i * kRowThreads];
     for (int j = 0; j < a.top; ++j) {
       const int row = a.slots[static_cast<int64_t>(t) * a.top + j];
       if (row < 0 || row >= rows) continue;
       Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(row) * packs;
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i)
+      for (int i = 0; i < kU; ++i)
         if (p0 + i * kRowThreads < packs) dst[p0 + i * kRowThreads] = v[i];
     }
   }
   zero_tail<T, N>(out, a.offsets, a.experts, rows, packs);
 }
 
-// combine (kWeighted) and gather_backward: a token's rows, weighted or not, added up.
+// combine (kWeighted) and gather_backward: a token's rows, weighted or not, added
+// up.  Four rows at a time: their places and weights first, then the loads of all
+// four together, then the sums in the order of the slots.
 template <typename T, int N, bool kWeighted>
 __global__ void __launch_bounds__(kRowThreads) moe_reduce_kernel(const MoeRowArgs a) {
   if (threadIdx.x == 0) pdl_allow_dependents();
   pdl_wait();
-  constexpr int kU = 2;
+  constexpr int kU = in_flight<T, N>(N * sizeof(T) == 16 ? 32 : 16), kJ = 4;
   const int packs = a.hidden / N;
   const int per_row = (packs + kRowThreads * kU - 1) / (kRowThreads * kU);
   const int64_t units = static_cast<int64_t>(a.tokens) * per_row;
@@ -243,73 +329,103 @@ __global__ void __launch_bounds__(kRowThreads) moe_reduce_kernel(const MoeRowArg
     for (int i = 0; i < kU; ++i)
 #pragma unroll
       for (int n = 0; n < N; ++n) acc[i][n] = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < a.top; ++j) {
-      const int64_t slot = static_cast<int64_t>(t) * a.top + j;
-      const int row = a.slots[slot];
-      if (row < 0 || row >= rows) continue;
-      const float w = kWeighted ? a.weights[slot] : 1.f;
-      const Pack<T, N>* src =
-          reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.in) + static_cast<int64_t>(row) * a.in_stride);
+    for (int j0 = 0; j0 < a.top; j0 += kJ) {
+      int row[kJ];
+      float w[kJ];
 #pragma unroll
-      for (int i = 0; i < kU; ++i)
-        if (p0 + i * kRowThreads < packs) {
-          const Pack<T, N> v = src[p0 + i * kRowThreads];
+      for (int j = 0; j < kJ; ++j) {
+        const int64_t slot = static_cast<int64_t>(t) * a.top + j0 + j;
+        row[j] = j0 + j < a.top ? a.slots[slot] : -1;
+        w[j] = kWeighted && j0 + j < a.top ? a.weights[slot] : 1.f;
+      }
+      Pack<T, N> v[kJ][kU];
 #pragma unroll
-          for (int n = 0; n < N; ++n) acc[i][n] = kWeighted ? fmaf(w, to_float(v.v[n]), acc[i][n]) : acc[i][n] + to_float(v.v[n]);
-        }
+      for (int j = 0; j < kJ; ++j) {
+        const Pack<T, N>* src = reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.in) +
+                                                                    static_cast<int64_t>(row[j]) * a.in_stride);
+#pragma unroll
+        for (int i = 0; i < kU; ++i)
+          if (row[j] >= 0 && row[j] < rows && p0 + i * kRowThreads < packs) v[j][i] = src[p0 + i * kRowThreads];
+      }
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+        if (row[j] >= 0 && row[j] < rows)
+#pragma unroll
+          for (int i = 0; i < kU; ++i)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+              acc[i][n] = kWeighted ? fmaf(w[j], v[j][i].get(n), acc[i][n]) : acc[i][n] + v[j][i].get(n);
     }
     Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(static_cast<T*>(a.out)) + static_cast<int64_t>(t) * packs;
 #pragma unroll
     for (int i = 0; i < kU; ++i)
       if (p0 + i * kRowThreads < packs) {
         Pack<T, N> v;
-#pragma unroll
-        for (int n = 0; n < N; ++n) put(v.v[n], acc[i][n]);
+        v.set(acc[i]);
         dst[p0 + i * kRowThreads] = v;
       }
   }
 }
 
-// A CTA takes one token: for each of its slots, dys = w * dy and the product
-// <dy, ys>, summed over the threads in a fixed order.
-template <typename T, int N>
+// kLanes threads take one slot: dys = w * dy and the product <dy, ys>, summed
+// over them in a fixed order.  A warp per slot where there are many (dy comes
+// from L1 for a token's other slots), a CTA per slot where there are few: 16
+// tokens of 8 slots and 7168 took 16.2 us with a CTA per token.
+template <typename T, int N, int kLanes>
 __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const MoeRowArgs a) {
+  static_assert(kLanes == 32 || kLanes == kRowThreads, "a warp or the CTA");
   __shared__ float part[kRowThreads / 32];
   if (threadIdx.x == 0) pdl_allow_dependents();
   pdl_wait();
+  constexpr int kU = in_flight<T, N>(64);
   const int packs = a.hidden / N;
   const int rows = a.tokens * a.top;
+  const int lane = threadIdx.x % kLanes;
   T* const out = static_cast<T*>(a.out);
-  for (int t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+  constexpr int kSlots = kRowThreads / kLanes;  // per CTA and step
+  for (int64_t slot = static_cast<int64_t>(blockIdx.x) * kSlots + threadIdx.x / kLanes; slot < rows;
+       slot += static_cast<int64_t>(gridDim.x) * kSlots) {
+    const int row = a.slots[slot];
+    if (row < 0 || row >= rows) {  // the same for all kLanes threads
+      if (lane == 0) a.dweights[slot] = 0.f;
+      continue;
+    }
+    const int64_t t = slot / a.top;
+    const float w = a.weights[slot];
     const Pack<T, N>* dy =
-        reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.grad) + static_cast<int64_t>(t) * a.grad_stride);
-    for (int j = 0; j < a.top; ++j) {
-      const int64_t slot = static_cast<int64_t>(t) * a.top + j;
-      const int row = a.slots[slot];
-      if (row < 0 || row >= rows) {  // the same for the whole CTA
-        if (threadIdx.x == 0) a.dweights[slot] = 0.f;
-        continue;
-      }
-      const float w = a.weights[slot];
-      const Pack<T, N>* ys =
-          reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.in) + static_cast<int64_t>(row) * a.in_stride);
-      Pack<T, N>* dys = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(row) * packs;
-      float dot = 0.f;
-#pragma unroll kUnroll
-      for (int p = threadIdx.x; p < packs; p += kRowThreads) {
-        const Pack<T, N> g = dy[p], v = ys[p];
-        Pack<T, N> d;
+        reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.grad) + t * a.grad_stride);
+    const Pack<T, N>* ys =
+        reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(a.in) + static_cast<int64_t>(row) * a.in_stride);
+    Pack<T, N>* dys = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(row) * packs;
+    float dot = 0.f;
+    for (int p0 = lane; p0 < packs; p0 += kLanes * kU) {
+      Pack<T, N> g[kU], v[kU];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const float gf = to_float(g.v[n]);
-          dot = fmaf(gf, to_float(v.v[n]), dot);
-          put(d.v[n], w * gf);
+      for (int i = 0; i < kU; ++i)
+        if (p0 + i * kLanes < packs) {
+          g[i] = dy[p0 + i * kLanes];
+          v[i] = ys[p0 + i * kLanes];
         }
-        dys[p] = d;
-      }
 #pragma unroll
-      for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      for (int i = 0; i < kU; ++i)
+        if (p0 + i * kLanes < packs) {
+          float scaled[N];
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            const float gf = g[i].get(n);
+            dot = fmaf(gf, v[i].get(n), dot);
+            scaled[n] = w * gf;
+          }
+          Pack<T, N> d;
+          d.set(scaled);
+          dys[p0 + i * kLanes] = d;
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    if (kLanes == 32) {
+      if (lane == 0) a.dweights[slot] = dot;
+    } else {
       if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = dot;
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -327,9 +443,11 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
 template <typename T, int N>
 cudaError_t launch_rows(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStream_t stream) {
   const int packs = a.hidden / N;
-  const int step = kRowThreads * (op == kMoeGather ? kUnroll : 2);
-  const int64_t units =
-      op == kMoeCombineBackward ? a.tokens : static_cast<int64_t>(a.tokens) * ((packs + step - 1) / step);
+  const int step = kRowThreads * in_flight<T, N>(op == kMoeGather ? 64 : N * sizeof(T) == 16 ? 32 : 16);
+  const int64_t slots = static_cast<int64_t>(a.tokens) * a.top;
+  const bool warps = op == kMoeCombineBackward && slots >= 8 * num_sms;  // enough for a warp each to fill the SMs
+  const int64_t units = op == kMoeCombineBackward ? (warps ? (slots + 3) / 4 : slots)
+                                                  : static_cast<int64_t>(a.tokens) * ((packs + step - 1) / step);
   const int64_t cap = static_cast<int64_t>(num_sms) * 16;
   const dim3 grid(static_cast<unsigned>(units < cap ? units : cap)), block(kRowThreads);
   switch (op) {
@@ -340,7 +458,8 @@ cudaError_t launch_rows(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStrea
     case kMoeCombine:
       return launch_pdl(moe_reduce_kernel<T, N, true>, grid, block, 0, stream, 1, a);
     default:
-      return launch_pdl(moe_combine_backward_kernel<T, N>, grid, block, 0, stream, 1, a);
+      return warps ? launch_pdl(moe_combine_backward_kernel<T, N, 32>, grid, block, 0, stream, 1, a)
+                   : launch_pdl(moe_combine_backward_kernel<T, N, kRowThreads>, grid, block, 0, stream, 1, a);
   }
 }
 
@@ -356,30 +475,36 @@ cudaError_t launch_type(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStrea
   return launch_rows<T, 1>(op, a, num_sms, stream);
 }
 
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t smem) {
+  if (smem <= 40 * 1024) return cudaSuccess;  // (with the static part under the default 48 KB)
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kMaxExperts * sizeof(int));
+}
+
 template <typename Id>
 cudaError_t launch_sort(const MoeSortArgs& a, int ctas, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(kSortWarps) * a.experts * sizeof(int);
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(moe_sort_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kSortWarps * kMaxExperts * sizeof(int));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(moe_count_kernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kSortWarps * kMaxExperts * sizeof(int));
-    if (e != cudaSuccess) return e;
+  cudaError_t e;
+  if (ctas == kSortCluster) {
+    if ((e = allow_smem(moe_sort_kernel<Id, true>, smem)) != cudaSuccess) return e;
+    return launch_pdl(moe_sort_kernel<Id, true>, dim3(ctas), dim3(kSortThreads), smem, stream, kSortCluster, a);
   }
+  if ((e = allow_smem(moe_sort_kernel<Id, false>, smem)) != cudaSuccess) return e;
   if (ctas > 1) {
-    cudaError_t e = launch_pdl(moe_count_kernel<Id>, dim3(ctas), dim3(kSortThreads), smem, stream, 1, a);
+    if ((e = allow_smem(moe_count_kernel<Id>, smem)) != cudaSuccess) return e;
+    e = launch_pdl(moe_count_kernel<Id>, dim3(ctas), dim3(kSortThreads), smem, stream, 1, a);
     if (e != cudaSuccess) return e;
   }
-  return launch_pdl(moe_sort_kernel<Id>, dim3(ctas), dim3(kSortThreads), smem, stream, 1, a);
+  return launch_pdl(moe_sort_kernel<Id, false>, dim3(ctas), dim3(kSortThreads), smem, stream, 1, a);
 }
 
-// CTAs for n slots: one up to 4096 (four passes of its 1024 threads: a second
-// launch and the counts' trip through memory cost more), then 2048 slots each,
-// at most one CTA per SM.
+// CTAs for n slots, by measured times (us): 512 slots 3.3 in one CTA and 4.1 in a
+// cluster, 2048 4.4 and 3.8; 32768 7.0 in a cluster and 6.5 in 32 CTAs with a second
+// launch, 131072 18.2 and 9.1; 524288 20.4 in 32 CTAs and 13.2 in 148.
 int sort_ctas(int n, int num_sms) {
-  if (n <= 4096) return 1;
-  const int c = (n + 2047) / 2048;
+  if (n <= 1024) return 1;
+  if (n <= 32768) return kSortCluster;
+  const int c = n / 4096 < 32 ? 32 : n / 4096;
   return c < num_sms ? c : num_sms;
 }
 
@@ -387,7 +512,7 @@ int sort_ctas(int n, int num_sms) {
 
 size_t moe_sort_workspace_bytes(int n, int experts, int num_sms) {
   const int c = sort_ctas(n, num_sms);
-  return c > 1 ? static_cast<size_t>(c) * experts * sizeof(int) : 0;
+  return c > kSortCluster ? static_cast<size_t>(c) * experts * sizeof(int) : 0;
 }
 
 cudaError_t launch_moe_sort(MoeSortArgs a, int num_sms, cudaStream_t stream) {

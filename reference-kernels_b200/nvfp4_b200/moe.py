@@ -182,7 +182,7 @@ def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, dow
     gate, up: operands (packed, scales) of [experts, N, H] weights, down of [experts, H, N], as mx.quantize makes them
     (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  The tokens and the gated values are
     quantised to MXFP4 on the way; x and the result are fp16, bf16 or fp32, and so are the values between the
-    products.  Six launches (seven for more than 4096 slots), no synchronisation."""
+    products.  Six launches (seven for more than 32768 slots), no synchronisation."""
     if gate[0].dim() != 3:
         _fail(f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
     routing = sort(ids, gate[0].shape[0])

@@ -19,7 +19,7 @@
 //   0, 10..12  TMA producers (K tiles of 256 dealt round-robin)
 //   1          TMEM owner, MMA issuer: tcgen05.mma kind::mxf4 block32, K = 64
 //   2..5, 13..16  epilogue: two groups of four, alternate steps of 32 tokens
-//   6..9, 17..20  scale writers, two sets for alternate K tiles: each tile's 128x4 scale blocks from shared memory
+//   6..9, 17..20  scale writers, for the even and the odd stages: each tile's 128x4 scale blocks from shared memory
 //              to TMEM (tcgen05.st; tcgen05.cp would take tensor-pipe time).  A
 //              token tile that begins inside a block of 128 takes its words from
 //              the block's middle on.
@@ -53,7 +53,6 @@ constexpr int kSfBytes = 1024;           // scales of 128 rows of one stage: two
 constexpr int kMaxProducers = 4;
 constexpr int kThreads = 672;
 constexpr int kGroups = 2;               // epilogue groups of four warps
-constexpr int kWriterSets = 2;
 constexpr int kMaxStages = 10;
 constexpr int kTmemCols = 512;
 constexpr int kChunk = 32;               // tokens per epilogue step
@@ -562,22 +561,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if ((warp >= 6 && warp <= 9) || warp >= 17) {
     // ------------------------------------------------------------ scale writers
-    // Two sets of four warps take alternate K tiles: one set's chain of wait, load,
-    // store and arrival took ~540 cycles a K tile, more than the MMAs.  Warp i
-    // writes lane quarter i % 4.  Columns of a stage: the
+    // Two sets of four warps, one for the even stages and one for the odd: one
+    // set's chain of wait, load, store and arrival took ~540 cycles a K tile, more
+    // than the MMAs.  (By stage and not by K tile: a set waits for a stage by phase
+    // parity, which is exact only if it has itself seen the stage's previous phase.
+    // With sets by K tile and an odd number of stages it has seen only every other
+    // one, and can take the phase before the last for its own.)  Warp i writes lane quarter i % 4.  Columns of a stage: the
     // weights' two blocks of 128 K columns (4 TMEM columns each), then the
     // tokens' (x_cols each); column c of an operand holds the words of its rows
     // 32 c .. 32 c + 31.
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    int e = 0, stage = warp >= 17 ? 1 : 0, ahead = stage;  // ahead: this set's next K tile, counted from the tile's first
+    const int set = warp >= 17 ? 1 : 0;
+    int e = 0, stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int t = t0; t < total && ok; t += step) {
       const Tile o = tile_at(p, tab, t, e);
       const int shift = o.in_blk >> 5;
       const int half = (feature0(o) & 127) >> 5;  // gated: the tile's first word in its weight blocks
-      int kt = k0 + ahead;
-      for (; kt < k1; kt += kWriterSets) {
+      for (int kt = k0; kt < k1; ++kt, ++stage) {
+        if (stage == S) {
+          stage = 0;
+          phase ^= 1;
+        }
+        if ((stage & 1) != set) continue;
         const bool got = mbar_wait(&sf_full[stage], phase);
         if (!__all_sync(0xffffffffu, got && !abort_flag)) {
           if (lane == 0 && !got) set_status(p.status, kStatusTimeoutFull);
@@ -659,13 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             mbar_arrive(&full[stage]);
         }
-        stage += kWriterSets;
-        if (stage >= S) {
-          stage -= S;
-          phase ^= 1;
-        }
       }
-      ahead = kt - k1;
     }
   }
 
@@ -969,7 +970,7 @@ struct Shape {
   double k_tile_us;
 };
 constexpr Shape kShapes[] = {{32, 0, 0.18}, {64, 0, 0.205}, {128, 0, 0.28},
-                             {128, 1, 0.24}, {192, 1, 0.29}, {256, 1, 0.43}};
+                             {128, 1, 0.24}, {192, 1, 0.29}, {256, 1, 0.39}};
 
 // The shape with the shortest rounds of tiles.  How unevenly a routing fills the
 // experts is not known here: tiles are counted for 0.6 .. 1.5 times the mean.
@@ -1032,12 +1033,6 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const int tmem_stages = (kTmemCols - p.acc_bufs * p.tn) / p.sf_cols;
   stages = stages < tmem_stages ? stages : tmem_stages;
   p.stages = stages < kMaxStages ? stages : kMaxStages;
-  // An even number: a stage then always belongs to the same set of scale
-  // writers.  A set waits for its stage by phase parity, which is exact only if
-  // it has itself seen the stage's previous phase; with an odd number it would
-  // find every other phase waited for by the other set, and could take the one
-  // before that for its own.
-  p.stages &= ~(kWriterSets - 1);
   // A producer waits on a stage by phase parity, which is exact only while it
   // waits for every stage at most one lap behind: not more producers than stages.
   p.producers = p.stages < kMaxProducers ? p.stages : kMaxProducers;

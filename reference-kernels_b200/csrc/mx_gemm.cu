@@ -217,10 +217,12 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3])
-               : "memory");
+// 16 bytes to another CTA's shared memory, counted on that CTA's barrier.
+__device__ __forceinline__ void st_async_v4(uint32_t addr, const uint32_t* v, uint32_t bar) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+      : "memory");
 }
 
 template <typename T>
@@ -306,6 +308,13 @@ __host__ __device__ constexpr int staging_bufs() {
   return sizeof(OutT) == 2 ? 2 : 1;
 }
 
+// kSplitK: groups of 8 tokens that a rank adds up, and its space for the others'
+// partial sums of them: 128 rows x 8 tokens in fp32 per group and rank.
+__host__ __device__ constexpr int rank_share(int groups, int splits) { return (groups + splits - 1) / splits; }
+__host__ __device__ constexpr int sums_bytes(int tn, int splits) {
+  return rank_share(tn / 8, splits) * (splits - 1) * 4096;
+}
+
 template <typename OutT, bool kGate, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
@@ -322,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
   constexpr int kBufs = staging_bufs<OutT>(), kStaged = kChunk * kF * sizeof(OutT);
   uint8_t* staging = smem + S * stage_bytes;  // per group kBufs of kStaged bytes (1024-aligned)
-  uint8_t* sfbuf = staging + kGroups * kBufs * kStaged;
+  uint8_t* sums = staging + kGroups * kBufs * kStaged;  // kSplit: the other ranks' partial sums
+  uint8_t* sfbuf = sums + (kSplit ? sums_bytes(p.tn, p.splits) : 0);
   uint4* exch = reinterpret_cast<uint4*>(sfbuf + S * sf_bytes);  // gated, per group: 512
   uint64_t* bars = reinterpret_cast<uint64_t*>(exch + (kGate ? kGroups * 512 : 0));
   uint64_t* full = bars;
@@ -331,7 +341,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_full = sf_full + S;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* sums_full = drain + 1;  // kSplit: the other ranks' partial sums are here
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sums_full + 1);
   int* row_tab = reinterpret_cast<int*>(tmem_slot + 2);
   int* blk_tab = row_tab + p.experts + 1;
   int* tile_tab = blk_tab + p.experts + 1;
@@ -352,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_empty[b], (kPair ? 2 : 1) * kGroups * 128);
     }
     mbar_init(drain, 1);
+    mbar_init(sums_full, 1);
     fence_barrier_init();
     prefetch_tensormap(&tm_w);
     prefetch_tensormap(&tm_x);
@@ -365,9 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       tmem_alloc(tmem_slot, kTmemCols);
   }
-  pdl_wait();
-  if (warp == 0) {
-    // Table of the experts, then the running number of their tiles.
+  // Table of the experts, then the running number of their tiles (warp 0).
+  auto build_table = [&]() {
     if (p.offsets) {
       load_expert_table(p.offsets, p.experts, p.rows, row_tab, blk_tab);
     } else if (lane == 0) {
@@ -389,13 +400,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       carry = __shfl_sync(0xffffffffu, n, 31);
     }
     if (lane == 0) tile_tab[0] = 0;
-  }
+  };
+  // What needs nothing of the kernel before runs while that one drains.
+  if (warp == 0 && !p.offsets) build_table();
   tc_fence_before();
-  if (kPair)
-    cluster_sync_all();  // both CTAs' barriers and TMEM are there
+  if (kPair || kSplit)
+    cluster_sync_all();  // the other CTAs' barriers and TMEM are there
   else
     __syncthreads();
   tc_fence_after();
+  pdl_wait();
+  if (p.offsets) {
+    if (warp == 0) build_table();
+    __syncthreads();
+  }
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t sf_col0 = p.acc_bufs * p.tn;
   const Table tab{row_tab, blk_tab, tile_tab};
@@ -832,53 +850,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int f = gtid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
   }
 
-  if (kSplit && t0 < total) {
+  if (kSplit) {
     // ---------------------------------------------------------- partial sums of a cluster
     // Groups of 8 tokens are dealt to the ranks in contiguous shares; each rank
     // sends its partial sums of the other ranks' shares to their shared memory
-    // (the pipeline's, free once every rank is past its main loop) and adds up
-    // its own share, own sums first and then by rank: the same order always.
-    // The epilogue groups take the even and the odd ones.
-    const bool ok = group >= 0 ? group_all(1 + group, partial_ready) : true;
+    // with st.async, which counts the bytes on the receiver's barrier, and adds
+    // up its own share, own sums first and then by rank: the same order always.
+    // The epilogue groups take the even and the odd ones.  (With two barriers of
+    // the cluster around plain stores the exchange took 2.0 us.)
+    const bool ok = group >= 0 ? group_all(1 + group, partial_ready) : false;
     tc_fence_after();
-    cluster_sync_all();
-    int e = 0;
-    const Tile o = tile_at(p, tab, t0, e);
-    const int ng = (o.rows + 7) >> 3;
-    const int share = (ng + p.splits - 1) / p.splits;
+    Tile o{};
+    int e = 0, ng = 0;
+    if (t0 < total) {
+      o = tile_at(p, tab, t0, e);
+      ng = (o.rows + 7) >> 3;
+    }
+    const int share = rank_share(ng, p.splits), first = rank * share, end = min(ng, first + share);
+    if (threadIdx.x == 64) mbar_arrive_expect_tx(sums_full, max(0, end - first) * (p.splits - 1) * 4096);
     const uint32_t tacc = tmem_base + tquarter;
     auto at = [&](int slot, int gi, int half) {
       return static_cast<uint32_t>((((slot * share + gi) * 2 + half) * 128 + gtid) * 16);
     };
-    if (group >= 0 && ok) {
+    if (ok) {
       constexpr int kAtOnce = 4;  // groups whose loads are in flight together
       for (int i = 1; i < p.splits; ++i) {
         const int peer = (rank + i) % p.splits;
-        const uint32_t base = map_peer(smem_u32(smem), peer);
+        const uint32_t base = map_peer(smem_u32(sums), peer), bar = map_peer(smem_u32(sums_full), peer);
         const int slot = rank < peer ? rank : rank - 1;
-        const int first = peer * share, end = min(ng, first + share);
-        for (int g0 = first + ((first ^ group) & 1); g0 < end; g0 += kGroups * kAtOnce) {
+        const int pfirst = peer * share, pend = min(ng, pfirst + share);
+        for (int g0 = pfirst + ((pfirst ^ group) & 1); g0 < pend; g0 += kGroups * kAtOnce) {
           uint32_t r[kAtOnce][8];
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k)
-            if (g0 + kGroups * k < end) {
+            if (g0 + kGroups * k < pend) {
               tmem_ld_16x256b_x1(tacc + 8 * (g0 + kGroups * k), r[k]);
               tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * (g0 + kGroups * k), r[k] + 4);
             }
           tmem_wait_ld();
 #pragma unroll
           for (int k = 0; k < kAtOnce; ++k)
-            if (g0 + kGroups * k < end) {
-              st_cluster_v4(base + at(slot, g0 + kGroups * k - first, 0), r[k]);
-              st_cluster_v4(base + at(slot, g0 + kGroups * k - first, 1), r[k] + 4);
+            if (g0 + kGroups * k < pend) {
+              st_async_v4(base + at(slot, g0 + kGroups * k - pfirst, 0), r[k], bar);
+              st_async_v4(base + at(slot, g0 + kGroups * k - pfirst, 1), r[k] + 4, bar);
             }
         }
       }
     }
-    cluster_sync_all();
-    if (group >= 0 && ok) {
-      const int first = rank * share;
-      for (int g = first + ((first ^ group) & 1); g < min(ng, first + share); g += kGroups) {
+    // No rank leaves before all have sent: whatever becomes of one rank's waits,
+    // nobody writes to the shared memory of a CTA that is gone.
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    if (ok && !group_all(1 + group, mbar_wait_cluster(sums_full, 0))) {
+      if (gtid == 0) set_status(p.status, kStatusTimeoutPeer);
+      abort_flag = 1;
+    } else if (ok) {
+      for (int g = first + ((first ^ group) & 1); g < end; g += kGroups) {
         uint32_t r[8];
         tmem_ld_16x256b_x1(tacc + 8 * g, r);
         tmem_ld_16x256b_x1(tacc + (16u << 16) + 8 * g, r + 4);
@@ -886,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int slot = 0; slot < p.splits - 1; ++slot)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float4 v = *reinterpret_cast<const float4*>(smem + at(slot, g - first, h));
+            const float4 v = *reinterpret_cast<const float4*>(sums + at(slot, g - first, h));
             r[4 * h] = __float_as_uint(__uint_as_float(r[4 * h]) + v.x);
             r[4 * h + 1] = __float_as_uint(__uint_as_float(r[4 * h + 1]) + v.y);
             r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
@@ -895,6 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         emit(std::integral_constant<int, 1>(), r, o.row0 + 8 * g, feature0(o), min(8, o.rows - 8 * g));
       }
     }
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
 
   if (group >= 0 && gtid == 0) bulk_wait_group0();  // C is written before the CTA ends
@@ -972,6 +999,25 @@ struct Shape {
 constexpr Shape kShapes[] = {{32, 0, 0.18}, {64, 0, 0.205}, {128, 0, 0.28},
                              {128, 1, 0.24}, {192, 1, 0.29}, {256, 1, 0.39}};
 
+// CTAs that share the K of each of at most `tiles` tiles.  One tile takes 4 + 0.18
+// us per K tile on its SM; sharing K costs some 1.5 us more for the exchange and
+// divides the rest until HBM is the limit (some 65 SMs).  Measured, one token:
+// 7168x16384 18.0 -> 15.4 us with 2 CTAs, 2048x7168 9.6 -> 7.3 with 4, 1024x16384
+// 16.9 -> 9.2 with 4 and 8.4 with 8 (clusters of 8 find room for few at a time: 16
+// of them took longer than 16 of 4); 4096x4096 7.1 -> 7.4 with 2.
+int k_splits(int64_t tiles, int KT, int num_sms) {
+  return tiles * 8 <= num_sms / 2 && KT >= 48 ? 8
+         : tiles * 4 <= num_sms && KT >= 24   ? 4
+         : tiles * 2 <= num_sms && KT >= 32   ? 2
+                                              : 1;
+}
+
+// Tiles at most, whatever the offsets.
+int64_t most_tiles(const MxGemmArgs& g, int tn, int busy, int n_tiles) {
+  return g.offsets ? (static_cast<int64_t>(g.rows) / tn + busy) * n_tiles
+                   : (static_cast<int64_t>(g.rows) + tn - 1) / tn * n_tiles;
+}
+
 // The shape with the shortest rounds of tiles.  How unevenly a routing fills the
 // experts is not known here: tiles are counted for 0.6 .. 1.5 times the mean.
 Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms) {
@@ -985,8 +1031,11 @@ Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms
       for (const double f : {0.6, 0.8, 1.0, 1.2, 1.5}) per_expert += std::ceil(f * mean / s.tn) / 5;
     else
       per_expert = std::ceil(mean / s.tn);
-    const double tiles = per_expert * busy * ((g.N + features - 1) / features);
-    const double us = std::ceil(tiles / (s.pair ? num_sms / 2 : num_sms)) * KT * s.k_tile_us;
+    const int n_tiles = (g.N + features - 1) / features;
+    const int splits = s.pair ? 1 : k_splits(most_tiles(g, s.tn, busy, n_tiles), KT, num_sms);
+    const double tiles = per_expert * busy * n_tiles;
+    const double us = splits > 1 ? KT * s.k_tile_us / splits + 1.5
+                                 : std::ceil(tiles / (s.pair ? num_sms / 2 : num_sms)) * KT * s.k_tile_us;
     if (us < best_us) {
       best = s;
       best_us = us;
@@ -1026,8 +1075,10 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.acc_bufs = p.tn <= 192 ? 2 : 1;
   p.x_cols = p.tn <= 128 ? 4 : p.tn / 32;
   p.sf_cols = 8 + 2 * p.x_cols;
+  const int64_t exact = most_tiles(g, p.tn, busy, p.n_tiles);
+  p.splits = p.pair ? 1 : k_splits(exact, KT, num_sms);
   // Stages: what shared memory and TMEM hold.
-  const size_t fixed = fixed_smem(out_size, gate, g.experts);
+  const size_t fixed = fixed_smem(out_size, gate, g.experts) + (p.splits > 1 ? sums_bytes(p.tn, p.splits) : 0);
   const size_t stage = kABytes + x_rows * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;
   int stages = static_cast<int>((kSmemMax - fixed) / stage);
   const int tmem_stages = (kTmemCols - p.acc_bufs * p.tn) / p.sf_cols;
@@ -1036,20 +1087,6 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   // A producer waits on a stage by phase parity, which is exact only while it
   // waits for every stage at most one lap behind: not more producers than stages.
   p.producers = p.stages < kMaxProducers ? p.stages : kMaxProducers;
-  // Tiles at most (whatever the offsets), and K splits where they leave SMs idle.
-  const int64_t tiles = (static_cast<int64_t>(g.rows) / p.tn + busy) * p.n_tiles;
-  const int64_t exact = g.offsets ? tiles : static_cast<int64_t>((g.rows + p.tn - 1) / p.tn) * p.n_tiles;
-  // One tile takes 4.4 + 0.17 us per K tile on its SM; sharing K costs 2.5 us more
-  // for the exchange and divides the rest until HBM is the limit (some 65 SMs).
-  // Measured, one token: 7168x16384 17.9 -> 16.0 us with 2 CTAs, 2048x7168
-  // 9.2 -> 8.1 with 4, 1024x16384 15.2 -> 10.0 with 4 and 8.8 with 8 (clusters of 8
-  // find room for few at a time: 16 of them took 14.5 us).
-  p.splits = 1;
-  if (!p.pair)
-    p.splits = exact * 8 <= num_sms / 2 && KT >= 48 ? 8
-               : exact * 4 <= num_sms && KT >= 24   ? 4
-               : exact * 2 <= num_sms && KT >= 32   ? 2
-                                                    : 1;
   const int64_t workers = p.pair ? num_sms / 2 : num_sms;
   const int64_t grid = p.splits > 1 ? exact * p.splits : (exact < workers ? exact : workers) * (p.pair ? 2 : 1);
   const size_t smem = fixed + p.stages * stage;

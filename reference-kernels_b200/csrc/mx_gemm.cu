@@ -76,6 +76,7 @@ struct Params {
   int splits;     // CTAs of a cluster that share a tile's K (kSplitK)
   int pair;       // kPairs
   int vec;        // 16-byte stores of C
+  int tma;        // TMA stores of C
   int* status;
   int inject;     // test hook: CTA 0 withholds its first weight load
 };
@@ -773,8 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     // A whole step, or the last rows of C, in TMA stores; the end of an expert's
-    // rows, and a C whose rows are not 16-byte aligned, by the threads.
-    const bool tma = G == 4 && p.vec && (valid == kChunk || row0 + valid == p.rows);
+    // rows, and a C whose rows do not begin and end at 16 bytes, by the threads.
+    const bool tma = G == 4 && p.tma && (valid == kChunk || row0 + valid == p.rows);
     if (tma) fence_proxy_async_smem();
     if (kBufs == 2 && gtid == 0) bulk_wait_group_read0();  // the other buffer, which the next step writes, is read
     bar_sync(1 + group, 128);
@@ -966,13 +967,13 @@ cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, 
       (kGate && !make_tma_3d_u8(&tw2, g.b2, k2, n, g.experts, k2, k2 * n, kBKBytes, wbox)) ||
       !make_tma_3d_u8(&tx, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kMode == kPairs ? p.tn / 2 : p.tn) ||
       !make_tma_3d_u8(&txs, g.a, k2, g.rows, 1, k2, k2 * g.rows, kBKBytes, kSmallBox) ||
-      (p.vec && !make_tma_3d_u8(&tc, g.c, n * sizeof(OutT), g.rows, 1, g.ldc * sizeof(OutT),
+      (p.tma && !make_tma_3d_u8(&tc, g.c, n * sizeof(OutT), g.rows, 1, g.ldc * sizeof(OutT),
                                 g.ldc * sizeof(OutT) * g.rows, 128, kChunk))) {
     *why = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
   return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kMode == kSplitK ? p.splits : kMode == kPairs ? 2 : 1, tw, kGate ? tw2 : tw, tx,
-                    txs, p.vec ? tc : tx, p);
+                    txs, p.tma ? tc : tx, p);
 }
 
 template <typename OutT>
@@ -1063,6 +1064,8 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.status = g.status;
   p.inject = g.inject;
   p.vec = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
+  // (A TMA store ends its rows at multiples of 16 bytes only.)
+  p.tma = p.vec && static_cast<int64_t>(g.N) * out_size % 16 == 0;
   const int KT = (g.K + kBK - 1) / kBK;
   const int busy = g.experts < g.rows ? g.experts : g.rows;
   const Shape shape = choose_shape(g, gate, KT, busy, num_sms);

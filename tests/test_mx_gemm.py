@@ -320,7 +320,37 @@ def test_two_streams_at_once_and_graphs():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(1, 128, 8192), (300, 256, 512)])
+@pytest.mark.parametrize("m,n,k", [(3000, 2100, 32), (3000, 2104, 288), (5000, 1000, 800), (700, 24, 64), (40, 8, 128),
+                                   (9000, 130, 544)])
+def test_more_tiles_than_sms_and_narrow_results(m, n, k):
+    """Many tiles of one to four K tiles in turn on each SM, and results narrower than a store's box."""
+    g = np.random.RandomState(m + n + k)
+    a, b = operand(m, k, g), operand(n, k, g)
+    same(mx.gemm(*on_gpu(*a), *on_gpu(*b)), mxref.decode(*a) @ mxref.decode(*b).T)
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,ldc,shift", [(70, 130, 256, 144, 0), (300, 64, 96, 72, 8), (33, 40, 64, 41, 1),
+                                             (1000, 4096, 64, 4112, 8), (1, 128, 8192, 136, 0)])
+def test_rows_of_c_apart(m, n, k, ldc, shift):
+    """C as part of a wider matrix through the C ABI: what lies beside it stays as it was."""
+    g = np.random.RandomState(m + n)
+    a, b = operand(m, k, g), operand(n, k, g)
+    (pa, sa), (pb, sb) = on_gpu(*a), on_gpu(*b)
+    c = torch.full((m + 1, ldc), 7.0, dtype=torch.bfloat16, device="cuda")
+    args = _lib.MxGemmArgs(pa.data_ptr(), pb.data_ptr(), None, sa.data_ptr(), sb.data_ptr(), None,
+                           c.data_ptr() + 2 * shift, None, m, n, k, 1, 1, 0, ldc,
+                           torch.cuda.current_stream().cuda_stream)
+    _lib.check(_lib.load().nvfp4_mx_gemm(ctypes.byref(args)))
+    flat = c.reshape(-1)[shift:shift + m * ldc].view(m, ldc)
+    same(flat[:, :n], mxref.decode(*a) @ mxref.decode(*b).T)
+    flat[:, :n] = 7.0
+    assert (c == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 128, 8192), (300, 256, 512), (600, 4096, 96), (1000, 4096, 1024)])
 def test_withheld_load_is_reported(monkeypatch, m, n, k):
     """A load that never comes ends in a status within the waits' limit, and the next call is right again."""
     g = np.random.RandomState(2)

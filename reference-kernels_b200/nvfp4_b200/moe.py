@@ -31,13 +31,36 @@ from .inputs import FP4X2
 from .mx import _DTYPES, _byref, _device, _experts, _fail, _launch, _raw_stream, E8M0, scale_blocks
 
 
-class Routing(NamedTuple):
-    """order int32 [T*top]: the slot (token * top + choice) of each sorted row, -1 behind the last;
-    slots int32 [T, top]: the sorted row of each slot, -1 where it is not routed;
-    offsets int32 [experts + 1]: each expert's first row, and the number of rows."""
+class _Lists(NamedTuple):
     order: torch.Tensor
     slots: torch.Tensor
     offsets: torch.Tensor
+
+
+class Routing(_Lists):
+    """order int32 [T*top]: the slot (token * top + choice) of each sorted row, -1 behind the last;
+    slots int32 [T, top]: the sorted row of each slot, -1 where it is not routed;
+    offsets int32 [experts + 1]: each expert's first row, and the number of rows.
+
+    Checked once, when it is made; tokens, top, experts and device (its CUDA index) are plain attributes."""
+
+    def __new__(cls, order, slots, offsets):
+        shape = slots.shape
+        if len(shape) != 2 or slots.dtype is not torch.int32 or not slots.is_contiguous():
+            _fail("moe.Routing: slots must be contiguous int32 [tokens, top]")
+        if order.dtype is not torch.int32 or order.shape != (shape[0] * shape[1],) or not order.is_contiguous():
+            _fail(f"moe.Routing: order must be contiguous int32 [{shape[0] * shape[1]}]")
+        self = super().__new__(cls, order, slots, offsets)
+        self.tokens, self.top = shape
+        self.experts = _experts("moe.Routing", offsets)
+        self.device = slots.get_device()
+        if order.get_device() != self.device or offsets.get_device() != self.device:
+            _fail("moe.Routing: order, slots and offsets must be on one device")
+        return self
+
+    @classmethod
+    def _make(cls, lists):
+        return cls(*lists)
 
 
 def sort(ids: torch.Tensor, experts: int) -> Routing:
@@ -63,16 +86,18 @@ def sort(ids: torch.Tensor, experts: int) -> Routing:
                             offsets.data_ptr(), work.data_ptr() if need else None, need, _raw_stream(dev))
     if rc:
         _lib.check(rc)
-    return Routing(order, slots, offsets)
+    routing = tuple.__new__(Routing, (order, slots, offsets))  # nothing to check
+    routing.tokens, routing.top = shape
+    routing.experts, routing.device = experts, dev
+    return routing
 
 
-def _check_routing(who: str, routing: Routing):
-    """(slots, offsets, tokens, top, experts) of a routing."""
-    _, slots, offsets = routing
-    shape = slots.shape
-    if len(shape) != 2 or slots.dtype is not torch.int32 or not slots.is_contiguous():
-        _fail(f"{who}: routing.slots must be contiguous int32 [tokens, top]")
-    return slots, offsets, shape[0], shape[1], _experts(who, offsets)
+def _on(who: str, routing: Routing, t: torch.Tensor, *others) -> int:
+    """The device of the routing and of every tensor, which has to be the current one."""
+    dev = _device(who, t, *others)
+    if routing.device != dev:
+        _fail(f"{who}: the routing is on cuda:{routing.device}, {who.split('.')[1]}'s tensors on cuda:{dev}")
+    return dev
 
 
 def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int):
@@ -89,18 +114,20 @@ def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int):
     return code, shape[1], stride
 
 
-def _check_weights(who: str, weights: torch.Tensor, slots: torch.Tensor) -> None:
-    if weights.dtype is not torch.float32 or weights.shape != slots.shape or not weights.is_contiguous():
-        _fail(f"{who}: weights must be contiguous fp32 {tuple(slots.shape)}, "
+def _check_weights(who: str, weights: torch.Tensor, routing: Routing) -> None:
+    want = (routing.tokens, routing.top)
+    if weights.dtype is not torch.float32 or weights.shape != want or not weights.is_contiguous():
+        _fail(f"{who}: weights must be contiguous fp32 {want}, "
               f"got {weights.dtype} {tuple(weights.shape)} (strides {weights.stride()})")
 
 
-def _rows(name, x, grad, weights, out, dweights, slots, offsets, code, tokens, top, h, experts, stride, gstride, dev):
+def _rows(name, routing, x, grad, weights, out, dweights, code, h, stride, gstride, dev):
     """One of the nvfp4_moe_* entry points that take nvfp4_moe_args."""
+    _, slots, offsets = routing
     rc = getattr(_lib.load(), name)(_byref(_lib.MoeArgs(
         x.data_ptr(), None if grad is None else grad.data_ptr(), None if weights is None else weights.data_ptr(),
         out.data_ptr(), None if dweights is None else dweights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), code,
-        tokens, top, h, experts, 0, stride, gstride, _raw_stream(dev))))
+        routing.tokens, routing.top, h, routing.experts, 0, stride, gstride, _raw_stream(dev))))
     if rc:
         _lib.check(rc)
 
@@ -108,53 +135,50 @@ def _rows(name, x, grad, weights, out, dweights, slots, offsets, code, tokens, t
 def gather(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """x [T, H] -> xs [T*top, H], each token's row at each of its sorted rows."""
     who = "moe.gather"
-    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    tokens = routing.tokens
     code, h, stride = _check_matrix(who, "x", x, tokens)
-    dev = _device(who, x, slots, offsets)
-    xs = x.new_empty((tokens * top, h))
-    _rows("nvfp4_moe_gather", x, None, None, xs, None, slots, offsets, code, tokens, top, h, experts, stride, 0, dev)
+    dev = _on(who, routing, x)
+    xs = x.new_empty((tokens * routing.top, h))
+    _rows("nvfp4_moe_gather", routing, x, None, None, xs, None, code, h, stride, 0, dev)
     return xs
 
 
 def gather_backward(dxs: torch.Tensor, routing: Routing) -> torch.Tensor:
     """The gradient of gather: dxs [T*top, H] -> dx [T, H], the sum over each token's rows."""
     who = "moe.gather_backward"
-    slots, offsets, tokens, top, experts = _check_routing(who, routing)
-    code, h, stride = _check_matrix(who, "dxs", dxs, tokens * top)
-    dev = _device(who, dxs, slots, offsets)
+    tokens = routing.tokens
+    code, h, stride = _check_matrix(who, "dxs", dxs, tokens * routing.top)
+    dev = _on(who, routing, dxs)
     dx = dxs.new_empty((tokens, h))
-    _rows("nvfp4_moe_gather_backward", dxs, None, None, dx, None, slots, offsets, code, tokens, top, h, experts,
-          stride, 0, dev)
+    _rows("nvfp4_moe_gather_backward", routing, dxs, None, None, dx, None, code, h, stride, 0, dev)
     return dx
 
 
 def combine(ys: torch.Tensor, weights: torch.Tensor, routing: Routing) -> torch.Tensor:
     """ys [T*top, H], weights fp32 [T, top] -> y [T, H], the weighted sum of each token's rows (no row: zeros)."""
     who = "moe.combine"
-    slots, offsets, tokens, top, experts = _check_routing(who, routing)
-    code, h, stride = _check_matrix(who, "ys", ys, tokens * top)
-    _check_weights(who, weights, slots)
-    dev = _device(who, ys, weights, slots, offsets)
+    tokens = routing.tokens
+    code, h, stride = _check_matrix(who, "ys", ys, tokens * routing.top)
+    _check_weights(who, weights, routing)
+    dev = _on(who, routing, ys, weights)
     y = ys.new_empty((tokens, h))
-    _rows("nvfp4_moe_combine", ys, None, weights, y, None, slots, offsets, code, tokens, top, h, experts, stride, 0,
-          dev)
+    _rows("nvfp4_moe_combine", routing, ys, None, weights, y, None, code, h, stride, 0, dev)
     return y
 
 
 def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, routing: Routing):
     """The gradients of combine: (dys [T*top, H], dweights fp32 [T, top])."""
     who = "moe.combine_backward"
-    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    tokens, rows = routing.tokens, routing.tokens * routing.top
     code, h, gstride = _check_matrix(who, "dy", dy, tokens)
-    ycode, yh, stride = _check_matrix(who, "ys", ys, tokens * top)
+    ycode, yh, stride = _check_matrix(who, "ys", ys, rows)
     if ycode != code or yh != h:
         _fail(f"{who}: ys must have dy's type and hidden size")
-    _check_weights(who, weights, slots)
-    dev = _device(who, dy, ys, weights, slots, offsets)
-    dys = ys.new_empty((tokens * top, h))
-    dweights = weights.new_empty((tokens, top))
-    _rows("nvfp4_moe_combine_backward", ys, dy, weights, dys, dweights, slots, offsets, code, tokens, top, h, experts,
-          stride, gstride, dev)
+    _check_weights(who, weights, routing)
+    dev = _on(who, routing, dy, ys, weights)
+    dys = ys.new_empty((rows, h))
+    dweights = weights.new_empty((tokens, routing.top))
+    _rows("nvfp4_moe_combine_backward", routing, ys, dy, weights, dys, dweights, code, h, stride, gstride, dev)
     return dys, dweights
 
 
@@ -162,11 +186,12 @@ def quantize_tokens(x: torch.Tensor, routing: Routing):
     """x [T, H] (fp16, bf16 or fp32, H % 32 == 0) -> the MXFP4 operand (packed [T*top, H/2], scales) of its sorted
     rows: mx.quantize of gather(x), with each token quantised once.  Rows behind the last expert's are not written."""
     who = "moe.quantize_tokens"
-    slots, offsets, tokens, top, experts = _check_routing(who, routing)
+    _, slots, offsets = routing
+    tokens, top, experts = routing.tokens, routing.top, routing.experts
     code, h, stride = _check_matrix(who, "x", x, tokens)
     if h == 0 or h % 32:
         _fail(f"{who}: hidden={h} must be a positive multiple of 32")
-    dev = _device(who, x, slots, offsets)
+    dev = _on(who, routing, x)
     rows = tokens * top
     packed = x.new_empty((rows, h // 2), dtype=FP4X2)
     scales = x.new_empty((scale_blocks(rows, experts), -(-h // 128), 32, 4, 4), dtype=E8M0)

@@ -8,8 +8,8 @@
 //   gather_backward   dx[token] = sum over its rows of dxs[row]
 //   combine           y[token] = sum over its slots of w[slot] * ys[row]
 //   combine_backward  dys[row] = w[slot] * dy[token],  dw[slot] = <dy[token], ys[row]>
-// Sums are held in fp32, in the order of the slots, and rounded once; nothing
-// is added with atomics, so results do not change from run to run.
+// Sums are held in fp32, in the order of the slots, and rounded once; no
+// value is added with atomics, so results do not change from run to run.
 //
 // All of them are bound by memory.  The work is split by token and not by row:
 // a token's own row is then read (gather, combine_backward) or written

@@ -282,7 +282,7 @@ template <typename T, int N>
 __global__ void __launch_bounds__(kRowThreads) moe_gather_kernel(const MoeRowArgs a) {
   if (threadIdx.x == 0) pdl_allow_dependents();
   pdl_wait();
-  constexpr int kU = in_flight<T, N>(64);
+  constexpr int kU = in_flight<T, N>(16);
   const int packs = a.hidden / N;
   const int per_row = (packs + kRowThreads * kU - 1) / (kRowThreads * kU);
   const int64_t units = static_cast<int64_t>(a.tokens) * per_row;
@@ -443,12 +443,14 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
 template <typename T, int N>
 cudaError_t launch_rows(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStream_t stream) {
   const int packs = a.hidden / N;
-  const int step = kRowThreads * in_flight<T, N>(op == kMoeGather ? 64 : N * sizeof(T) == 16 ? 32 : 16);
+  const int step = kRowThreads * in_flight<T, N>(op != kMoeGather && N * sizeof(T) == 16 ? 32 : 16);
   const int64_t slots = static_cast<int64_t>(a.tokens) * a.top;
   const bool warps = op == kMoeCombineBackward && slots >= 8 * num_sms;  // enough for a warp each to fill the SMs
   const int64_t units = op == kMoeCombineBackward ? (warps ? (slots + 3) / 4 : slots)
                                                   : static_cast<int64_t>(a.tokens) * ((packs + step - 1) / step);
-  const int64_t cap = static_cast<int64_t>(num_sms) * 16;
+  // (64 CTAs of 128 threads per SM against 16, 8192 tokens to 4 experts each, bf16,
+  // 4096: gather 62 -> 55 us, combine 55 -> 52, its gradient 97 -> 93.)
+  const int64_t cap = static_cast<int64_t>(num_sms) * 64;
   const dim3 grid(static_cast<unsigned>(units < cap ? units : cap)), block(kRowThreads);
   switch (op) {
     case kMoeGather:

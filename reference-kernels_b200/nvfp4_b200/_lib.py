@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # NVFP4_B200_LIBRARY points at another build of the same C ABI (e.g. a variant
@@ -85,6 +86,13 @@ class MoeArgs(ctypes.Structure):
                 ("in_stride", _L), ("grad_stride", _L), ("stream", _P)]
 
 
+# The same three structs as bytes in one call, for the calls of a few microseconds: filling a ctypes.Structure of as
+# many fields takes four times as long.  A null pointer is 0.
+pack_mx_quant = struct.Struct("@5P6i2qP").pack
+pack_mx_gemm = struct.Struct("@8P6iqP").pack
+pack_moe = struct.Struct("@7P6i2qP").pack
+
+
 class Nvfp4Error(RuntimeError):
     """Raised when an entry point of libnvfp4_b200.so returns a non-zero code."""
 
@@ -121,18 +129,15 @@ def load() -> ctypes.CDLL:
     for name in ("nvfp4_gemm_call", "nvfp4_dual_gemm_call"):
         getattr(lib, name).restype = _I
         getattr(lib, name).argtypes = [ctypes.POINTER(GemmArgs)]
-    for name in ("nvfp4_mx_quantize", "nvfp4_mx_dequantize"):
+    # Packed bytes, or byref of the struct.
+    for name in ("nvfp4_mx_quantize", "nvfp4_mx_dequantize", "nvfp4_mx_gemm", "nvfp4_moe_gather",
+                 "nvfp4_moe_gather_backward", "nvfp4_moe_combine", "nvfp4_moe_combine_backward"):
         getattr(lib, name).restype = _I
-        getattr(lib, name).argtypes = [ctypes.POINTER(MxQuantArgs)]
-    lib.nvfp4_mx_gemm.restype = _I
-    lib.nvfp4_mx_gemm.argtypes = [ctypes.POINTER(MxGemmArgs)]
+        getattr(lib, name).argtypes = [_P]
     lib.nvfp4_moe_sort_workspace.restype = _L
     lib.nvfp4_moe_sort_workspace.argtypes = [_I, _I]
     lib.nvfp4_moe_sort.restype = _I
     lib.nvfp4_moe_sort.argtypes = [_P, _I, _I, _I, _P, _P, _P, _P, _L, _P]
-    for name in ("nvfp4_moe_gather", "nvfp4_moe_gather_backward", "nvfp4_moe_combine", "nvfp4_moe_combine_backward"):
-        getattr(lib, name).restype = _I
-        getattr(lib, name).argtypes = [ctypes.POINTER(MoeArgs)]
     _lib = lib
     return lib
 

@@ -28,7 +28,7 @@ import torch
 
 from . import _lib, mx
 from .inputs import FP4X2
-from .mx import _DTYPES, _byref, _device, _experts, _fail, _launch, _raw_stream, E8M0, scale_blocks
+from .mx import _DTYPES, _device, _experts, _fail, _launch, _raw_stream, E8M0, scale_blocks
 
 
 class _Lists(NamedTuple):
@@ -42,20 +42,19 @@ class Routing(_Lists):
     slots int32 [T, top]: the sorted row of each slot, -1 where it is not routed;
     offsets int32 [experts + 1]: each expert's first row, and the number of rows.
 
-    Checked once, when it is made; tokens, top, experts and device (its CUDA index) are plain attributes."""
+    slots and offsets are checked once, when it is made (order is for the caller: nothing here reads it); tokens,
+    top, experts and device (its CUDA index) are plain attributes."""
 
     def __new__(cls, order, slots, offsets):
         shape = slots.shape
         if len(shape) != 2 or slots.dtype is not torch.int32 or not slots.is_contiguous():
             _fail("moe.Routing: slots must be contiguous int32 [tokens, top]")
-        if order.dtype is not torch.int32 or order.shape != (shape[0] * shape[1],) or not order.is_contiguous():
-            _fail(f"moe.Routing: order must be contiguous int32 [{shape[0] * shape[1]}]")
-        self = super().__new__(cls, order, slots, offsets)
+        self = tuple.__new__(cls, (order, slots, offsets))
         self.tokens, self.top = shape
         self.experts = _experts("moe.Routing", offsets)
         self.device = slots.get_device()
-        if order.get_device() != self.device or offsets.get_device() != self.device:
-            _fail("moe.Routing: order, slots and offsets must be on one device")
+        if offsets.get_device() != self.device:
+            _fail("moe.Routing: slots and offsets must be on one device")
         return self
 
     @classmethod
@@ -124,10 +123,10 @@ def _check_weights(who: str, weights: torch.Tensor, routing: Routing) -> None:
 def _rows(name, routing, x, grad, weights, out, dweights, code, h, stride, gstride, dev):
     """One of the nvfp4_moe_* entry points that take nvfp4_moe_args."""
     _, slots, offsets = routing
-    rc = getattr(_lib.load(), name)(_byref(_lib.MoeArgs(
-        x.data_ptr(), None if grad is None else grad.data_ptr(), None if weights is None else weights.data_ptr(),
-        out.data_ptr(), None if dweights is None else dweights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), code,
-        routing.tokens, routing.top, h, routing.experts, 0, stride, gstride, _raw_stream(dev))))
+    rc = getattr(_lib.load(), name)(_lib.pack_moe(
+        x.data_ptr(), 0 if grad is None else grad.data_ptr(), 0 if weights is None else weights.data_ptr(),
+        out.data_ptr(), 0 if dweights is None else dweights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), code,
+        routing.tokens, routing.top, h, routing.experts, 0, stride, gstride, _raw_stream(dev)))
     if rc:
         _lib.check(rc)
 

@@ -22,8 +22,6 @@ can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -35,7 +33,6 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
-_byref = ctypes.byref
 
 
 def _fail(msg: str):
@@ -152,10 +149,10 @@ def quantize(x: torch.Tensor, axis: int = -1, offsets: torch.Tensor | None = Non
 
 def _launch(name, x, packed, scales, offsets, slots, dtype, rows, k, experts, top, columns, rstride, estride, dev):
     """nvfp4_mx_quantize or nvfp4_mx_dequantize."""
-    rc = getattr(_lib.load(), name)(_byref(_lib.MxQuantArgs(
-        x.data_ptr(), packed.data_ptr(), scales.data_ptr(), None if offsets is None else offsets.data_ptr(),
-        None if slots is None else slots.data_ptr(), dtype, rows, k, experts, top, columns, rstride, estride,
-        _raw_stream(dev))))
+    rc = getattr(_lib.load(), name)(_lib.pack_mx_quant(
+        x.data_ptr(), packed.data_ptr(), scales.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+        0 if slots is None else slots.data_ptr(), dtype, rows, k, experts, top, columns, rstride, estride,
+        _raw_stream(dev)))
     if rc:
         _lib.check(rc)
 
@@ -201,10 +198,10 @@ def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype):
     c = a.new_empty((rows, n), dtype=out_dtype)
     if rows and n:
         gated = b2 is not None
-        rc = _lib.load().nvfp4_mx_gemm(_byref(_lib.MxGemmArgs(
-            a.data_ptr(), b1.data_ptr(), b2.data_ptr() if gated else None, sa.data_ptr(), s1.data_ptr(),
-            s2.data_ptr() if gated else None, c.data_ptr(), None if offsets is None else offsets.data_ptr(), rows, n,
-            2 * k2, experts or 1, code, 0, n, _raw_stream(dev))))
+        rc = _lib.load().nvfp4_mx_gemm(_lib.pack_mx_gemm(
+            a.data_ptr(), b1.data_ptr(), b2.data_ptr() if gated else 0, sa.data_ptr(), s1.data_ptr(),
+            s2.data_ptr() if gated else 0, c.data_ptr(), 0 if offsets is None else offsets.data_ptr(), rows, n,
+            2 * k2, experts or 1, code, 0, n, _raw_stream(dev)))
         if rc:
             _lib.check(rc)
         if _CHECK_STATUS:

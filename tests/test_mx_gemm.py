@@ -112,6 +112,13 @@ def test_struct_layout_matches_header(tmp_path):
     assert got == want
 
 
+def test_packed_bytes_equal_the_structs():
+    for py, pack, n in [(_lib.MxQuantArgs, _lib.pack_mx_quant, 14), (_lib.MxGemmArgs, _lib.pack_mx_gemm, 16),
+                        (_lib.MoeArgs, _lib.pack_moe, 16)]:
+        values = [3 * i + 1 for i in range(n)]
+        assert bytes(py(*values)) == pack(*values)
+
+
 # ---------------------------------------------------------------- GPU: one matrix
 SIZES = [(1, 1, 32), (1, 128, 256), (5, 7, 64), (31, 130, 96), (33, 64, 160), (64, 257, 1024), (100, 300, 544),
          (130, 128, 7168), (193, 200, 288), (256, 129, 512), (385, 640, 320), (1000, 384, 736), (2049, 72, 128),

@@ -16,13 +16,25 @@
 // an output share a tile, its token operand and its accumulator.
 //
 // One persistent CTA per SM, 21 warps:
-//   0, 10..12  TMA producers (K tiles of 256 dealt round-robin)
-//   1          TMEM owner, MMA issuer: tcgen05.mma kind::mxf4 block32, K = 64
-//   2..5, 13..16  epilogue: two groups of four, alternate steps of 32 tokens
-//   6..9, 17..20  scale writers, for the even and the odd stages: each tile's 128x4 scale blocks from shared memory
-//              to TMEM (tcgen05.st; tcgen05.cp would take tensor-pipe time).  A
-//              token tile that begins inside a block of 128 takes its words from
-//              the block's middle on.
+//   0, 10..12      TMA producers (K tiles of 256 dealt round-robin)
+//   1              TMEM owner, MMA issuer: tcgen05.mma kind::mxf4 block32, K = 64
+//   2..5, 13..16   epilogue: two groups of four, alternate steps of 32 tokens
+//   6..9, 17..20   scale writers, for the even and the odd stages: each tile's
+//                  128x4 scale blocks from shared memory to TMEM (tcgen05.st;
+//                  tcgen05.cp would take tensor-pipe time).  A token tile that
+//                  begins inside a block of 128 takes its words from the block's
+//                  middle on.
+// Over 128 tokens, pairs of CTAs (cta_group::2): 256 weight rows, each CTA with its
+// own half of them and of the tokens, which halves the token bytes per SM.
+//
+// What bounds it, on B200: few tokens by HBM -- 32 tokens over 64 experts, gated,
+// 2048x4096: 77 us for 0.56 GB, 7.3 TB/s, above the 6.6 TB/s of a copy; one token
+// through 7168x16384 15.4 us, 9.5 of them traffic, the rest set-up, the first
+// loads' latency and the exchange of partial sums.  Many tokens by what an SM
+// takes from L2: a pair's 192-token tile needs 31 KB per 384 cycles of MMA, and
+// 57 bytes a clock arrive of the 64 that an SM's port has -- 1000x7168x16384 48 us
+// (4.9 PFLOP/s), 8192x7168x4096 98 us, 8192x7168x16384 329 us (5.85 PFLOP/s, 0.87
+// of 4 x the measured bf16 rate).  Over seconds the power cap takes 15 % of that.
 // The offsets are read on the device: every CTA builds the table of the experts'
 // rows, scale blocks and tiles in shared memory and walks the same tile list, so
 // the host never waits for a routing.
@@ -274,8 +286,8 @@ __device__ __forceinline__ Tile uniform(const Tile& o) {
 
 // Tile t (< tab.tile[E]); `e` is the walker's cursor.  Tiles of an expert go
 // over up to kGroup token tiles for each weight tile, so that CTAs that run
-// together share both operands in L2.
-constexpr int kGroup = 12;
+// together share both operands in L2 (24 against 12: 8192x7168x4096 100 -> 98 us).
+constexpr int kGroup = 24;
 __device__ __forceinline__ Tile tile_at(const Params& p, const Table& tab, int t, int& e) {
   while (t >= tab.tile[e + 1]) ++e;
   const int count = tab.row[e + 1] - tab.row[e];

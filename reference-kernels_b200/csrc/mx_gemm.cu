@@ -603,19 +603,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     // 32 c .. 32 c + 31.
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int set = warp >= 17 ? 1 : 0;
-    int e = 0, stage = 0;
+    int e = 0, stage = set, ahead = set;  // ahead: this set's next K tile, counted from the tile's first
     uint32_t phase = 0;
     bool ok = true;
     for (int t = t0; t < total && ok; t += step) {
       const Tile o = tile_at(p, tab, t, e);
       const int shift = o.in_blk >> 5;
       const int half = (feature0(o) & 127) >> 5;  // gated: the tile's first word in its weight blocks
-      for (int kt = k0; kt < k1; ++kt, ++stage) {
-        if (stage == S) {
-          stage = 0;
-          phase ^= 1;
-        }
-        if ((stage & 1) != set) continue;
+      int kt = k0 + ahead;
+      while (kt < k1) {
         const bool got = mbar_wait(&sf_full[stage], phase);
         if (!__all_sync(0xffffffffu, got && !abort_flag)) {
           if (lane == 0 && !got) set_status(p.status, kStatusTimeoutFull);
@@ -697,7 +693,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             mbar_arrive(&full[stage]);
         }
+        if (stage + 2 < S) {
+          stage += 2;
+          kt += 2;
+        } else {  // on to the set's first stage of the next lap
+          kt += S - stage + set;
+          stage = set;
+          phase ^= 1;
+        }
       }
+      ahead = kt - k1;
     }
   }
 

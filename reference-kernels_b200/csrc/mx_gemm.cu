@@ -41,6 +41,10 @@
 //
 // Few tiles (a decoding step of one matrix): a cluster splits K and adds its
 // partial sums through distributed shared memory, in rank order.
+//
+// Every wait is bounded.  A role whose wait runs out records it and stops; the
+// others then run out of what it would have given them, within a second each.  (A
+// flag that all of them read at every K tile cost 2 %.)
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -69,7 +73,7 @@ constexpr int kMaxStages = 10;
 constexpr int kTmemCols = 512;
 constexpr int kChunk = 32;               // tokens per epilogue step
 constexpr int kSmallBox = 32;            // token rows of a small TMA box
-constexpr int kSmemMax = 227 * 1024 - 128;  // dynamic; the rest is for the static abort flag
+constexpr int kSmemMax = 227 * 1024;
 
 struct Params {
   const uint8_t* sfw;   // scales of the weights (b, b1)
@@ -359,13 +363,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* row_tab = reinterpret_cast<int*>(tmem_slot + 2);
   int* blk_tab = row_tab + p.experts + 1;
   int* tile_tab = blk_tab + p.experts + 1;
-  __shared__ volatile int abort_flag;
-
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int KT = (p.K + kBK - 1) / kBK, K128 = (p.K + 127) >> 7;
 
   if (threadIdx.x == 0) {
-    abort_flag = 0;
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], kPair ? 1 + 8 : 1 + 4);  // the producer, and each scale writer (of both CTAs)
       mbar_init(&empty[s], 1);
@@ -478,9 +479,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tx = (kABytes + boxes * box_bytes) * (kPair ? 2 : 1);
         int kt = k0 + ahead;
         for (; kt < k1; kt += P) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase) && !abort_flag)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase))) {
             if (issue) set_status(p.status, kStatusTimeoutEmpty);
-            abort_flag = 1;
             ok = false;
             break;
           }
@@ -534,7 +534,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = __shfl_sync(0xffffffffu, (tile_at(p, tab, t, e).rows + 31) & ~31, 0);
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[acc], acc_phase ^ 1))) {
           if (issue) set_status(p.status, kStatusTimeoutAccEmpty);
-          abort_flag = 1;
           break;
         }
         tc_fence_after();
@@ -543,7 +542,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int kt = k0; kt < k1; ++kt) {
           if (!__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(&full[stage], phase) : mbar_wait(&full[stage], phase))) {
             if (issue) set_status(p.status, kStatusTimeoutFull);
-            abort_flag = 1;
             ok = false;
             break;
           }
@@ -597,10 +595,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // than the MMAs.  (By stage and not by K tile: a set waits for a stage by phase
     // parity, which is exact only if it has itself seen the stage's previous phase.
     // With sets by K tile and an odd number of stages it has seen only every other
-    // one, and can take the phase before the last for its own.)  Warp i writes lane quarter i % 4.  Columns of a stage: the
-    // weights' two blocks of 128 K columns (4 TMEM columns each), then the
-    // tokens' (x_cols each); column c of an operand holds the words of its rows
-    // 32 c .. 32 c + 31.
+    // one, and can take the phase before the last for its own.)  Warp i writes
+    // lane quarter i % 4.  Columns of a stage: the weights' two blocks of 128 K
+    // columns (4 TMEM columns each), then the tokens' (x_cols each); column c of an
+    // operand holds the words of its rows 32 c .. 32 c + 31.
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int set = warp >= 17 ? 1 : 0;
     int e = 0, stage = set, ahead = set;  // ahead: this set's next K tile, counted from the tile's first
@@ -612,10 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int half = (feature0(o) & 127) >> 5;  // gated: the tile's first word in its weight blocks
       int kt = k0 + ahead;
       while (kt < k1) {
-        const bool got = mbar_wait(&sf_full[stage], phase);
-        if (!__all_sync(0xffffffffu, got && !abort_flag)) {
-          if (lane == 0 && !got) set_status(p.status, kStatusTimeoutFull);
-          abort_flag = 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sf_full[stage], phase))) {
+          if (lane == 0) set_status(p.status, kStatusTimeoutFull);
           ok = false;
           break;
         }
@@ -832,7 +828,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The four warps agree before any goes on to the named barriers.
       if (!group_all(1 + group, mbar_wait(&acc_full[acc], acc_phase))) {
         if (gtid == 0) set_status(p.status, kStatusTimeoutAccFull);
-        abort_flag = 1;
         break;
       }
       tc_fence_after();
@@ -920,7 +915,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     if (ok && !group_all(1 + group, mbar_wait_cluster(sums_full, 0))) {
       if (gtid == 0) set_status(p.status, kStatusTimeoutPeer);
-      abort_flag = 1;
     } else if (ok) {
       for (int g = first + ((first ^ group) & 1); g < end; g += kGroups) {
         uint32_t r[8];

@@ -76,21 +76,38 @@ struct Block {
   static constexpr int kWords = 8 * sizeof(T);
   uint32_t w[kWords];
 
-  // kAlign: bytes that the address is a multiple of: 32, 16, or a type's own.
+  // kAlign: bytes that the address is a multiple of, 32 or 16.
   template <int kAlign>
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kAlign == 32) {
 #pragma unroll
       for (int i = 0; i < kWords / 8; ++i) load32(reinterpret_cast<const uint32_t*>(p) + 8 * i, w + 8 * i);
-    } else if constexpr (kAlign == 16) {
+    } else {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i)
         *reinterpret_cast<uint4*>(w + 4 * i) = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    } else {
-      T* t = reinterpret_cast<T*>(w);
-#pragma unroll
-      for (int i = 0; i < 32; ++i) t[i] = p[i];
     }
+  }
+  // Any address: the warp loads its lanes' blocks one after another, an element
+  // per lane and all in flight, and deals them out through `rows` of shared memory.
+  // (4096 x 4096 in bf16: 15.8 us, 35 with each lane loading its own elements; 6.5
+  // for aligned rows.)
+  static constexpr int kPitch = 32 + 4 / static_cast<int>(sizeof(T));  // elements; an odd number of words
+  __device__ __forceinline__ void load_any(const T* p, bool active, T (*rows)[kPitch]) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t with = __ballot_sync(0xffffffffu, active);
+    __syncwarp();  // the last step's rows are read
+    T v[32];
+#pragma unroll
+    for (int b = 0; b < 32; ++b) {
+      const T* q = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), b));
+      v[b] = with >> b & 1 ? q[lane] : T(0.f);
+    }
+#pragma unroll
+    for (int b = 0; b < 32; ++b) rows[b][lane] = v[b];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint32_t*>(rows[lane])[i];
   }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (std::is_same<T, float>::value) {
@@ -188,7 +205,13 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const MxQuantArgs
       scale_row = static_cast<int64_t>(e) * ((a.rows_per + 127) >> 7) * 128 + i;
     }
     Block<T> x;
-    if (active) x.template load<kAlign>(static_cast<const T*>(a.x) + src + 32 * j);
+    const T* const p = static_cast<const T*>(a.x) + src + 32 * j;
+    if constexpr (kAlign == 1) {
+      __shared__ alignas(16) T rows[kWarps][32][Block<T>::kPitch];
+      x.load_any(p, active, rows[threadIdx.x >> 5]);
+    } else {
+      if (active) x.template load<kAlign>(p);
+    }
     if (kMode == 1) {
       scale_row = f < total ? sorted_scale_row(tab, a.experts, r) : -1;
       active = active && scale_row >= 0;

@@ -86,15 +86,26 @@ class MoeArgs(ctypes.Structure):
                 ("in_stride", _L), ("grad_stride", _L), ("stream", _P)]
 
 
-# The same three structs as bytes in one call, for the calls of a few microseconds: filling a ctypes.Structure of as
-# many fields takes four times as long.  A null pointer is 0.
-pack_mx_quant = struct.Struct("@5P6i2qP").pack
-pack_mx_gemm = struct.Struct("@8P6iqP").pack
-pack_moe = struct.Struct("@7P6i2qP").pack
-
-
 class Nvfp4Error(RuntimeError):
     """Raised when an entry point of libnvfp4_b200.so returns a non-zero code."""
+
+
+def _packer(layout: str):
+    pack = struct.Struct(layout).pack
+
+    def packed(*values) -> bytes:
+        try:
+            return pack(*values)
+        except struct.error:
+            raise Nvfp4Error(f"a size does not fit the C interface's 32-bit integers: {values}") from None
+    return packed
+
+
+# The last three structs as bytes in one call, for calls of a few microseconds: filling a ctypes.Structure of as many
+# fields takes four times as long.  A null pointer is 0.
+pack_mx_quant = _packer("@5P6i2qP")
+pack_mx_gemm = _packer("@8P6iqP")
+pack_moe = _packer("@7P6i2qP")
 
 
 def load() -> ctypes.CDLL:

@@ -72,6 +72,8 @@ def sort(ids: torch.Tensor, experts: int) -> Routing:
         _fail(f"{who}: ids must be contiguous [tokens, top], got {tuple(shape)} (strides {ids.stride()})")
     dev = _device(who, ids)
     n = shape[0] * shape[1]
+    if n >= 1 << 31:
+        _fail(f"{who}: {n} slots do not fit 32-bit rows")
     lib = _lib.load()
     need = lib.nvfp4_moe_sort_workspace(n, experts)
     if need < 0:

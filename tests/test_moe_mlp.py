@@ -105,6 +105,16 @@ def test_mlp_steps_are_its_own_operators_and_it_can_be_captured():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,top", [(0, 2), (5, 0), (5, 2)])
+def test_mlp_without_routed_tokens(tokens, top):
+    _, _, _, (gate, _), (up, _), (down, _) = layer(1, 1, 3, 64, 96, torch.bfloat16, 2)
+    x = torch.ones((tokens, 64), dtype=torch.bfloat16, device="cuda")
+    ids = torch.full((tokens, top), -1, device="cuda")
+    y = moe.mlp(x, ids, torch.ones((tokens, top), device="cuda"), gate, up, down)
+    assert y.shape == (tokens, 64) and not y.any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens,n,k", [(70, 96, 64), (257, 130, 200), (512, 384, 256)])
 def test_linear_layer_forward_and_gradients(tokens, n, k):
     """y = x w^T, dx = dy w, dw = dy^T x, each with both operands in MXFP4 along its own sum (axis=0 quantises along

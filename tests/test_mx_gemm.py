@@ -117,6 +117,8 @@ def test_packed_bytes_equal_the_structs():
                         (_lib.MoeArgs, _lib.pack_moe, 16)]:
         values = [3 * i + 1 for i in range(n)]
         assert bytes(py(*values)) == pack(*values)
+        with pytest.raises(_lib.Nvfp4Error, match="32-bit"):
+            pack(*[1 << 31] * n)
 
 
 # ---------------------------------------------------------------- GPU: one matrix

@@ -235,12 +235,14 @@ typedef struct {
 int nvfp4_mx_quantize(const nvfp4_mx_quant_args* args);
 int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* args);
 
-/* Products of MXFP4 operands, fp32 sums, out_dtype 0 (fp16), 1 (bf16), 2 (fp32):
+/* Products of MXFP4 operands, fp32 sums, out_dtype 0 (fp16), 1 (bf16), 2 (fp32), 3 (MXFP4):
  *   c[r, n] = sum_k a[r, k] b[e(r)][n, k],   or, with b2 and its scales,
  *   c[r, n] = silu(a[r] . b[e(r)][n]) * (a[r] . b2[e(r)][n])
  *   a       : codes [rows][K/2], scales as above
  *   b, b2   : codes [experts][N][K/2], scales [experts][ceil(N/128)] row blocks
- *   c       : [rows][ldc]
+ *   c       : [rows][ldc]; with out_dtype 3 (b2 only, N % 32 == 0) the codes
+ *             [rows][N/2] of the fp32 result as nvfp4_mx_quantize would make them
+ *             with the same offsets, and their scales in c_scales
  *   offsets : the rows are sorted by expert; NULL with experts == 1
  * Any rows >= 0 and N >= 1, K % 32 == 0.  Needs no workspace: calls on several
  * streams may overlap. */
@@ -252,6 +254,7 @@ typedef struct {
   const void* sfb;
   const void* sfb2;
   void* c;
+  void* c_scales;
   const int32_t* offsets;
   int32_t rows, N, K, experts, out_dtype, reserved;
   int64_t ldc;

@@ -479,26 +479,30 @@ NVFP4_API int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* x) {
 NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
   const char* name = "nvfp4_mx_gemm";
   if (!x) return fail(NVFP4_ERR_NULL, "%s: null argument block", name);
-  if (x->out_dtype < 0 || x->out_dtype > 2)
-    return fail(NVFP4_ERR_SHAPE, "%s: out_dtype must be 0 (fp16), 1 (bf16) or 2 (fp32)", name);
+  if (x->out_dtype < 0 || x->out_dtype > 3)
+    return fail(NVFP4_ERR_SHAPE, "%s: out_dtype must be 0 (fp16), 1 (bf16), 2 (fp32) or 3 (MXFP4)", name);
+  const bool codes = x->out_dtype == 3;
   if (x->rows < 0 || x->N <= 0 || x->K <= 0 || x->experts < 1)
     return fail(NVFP4_ERR_SHAPE, "%s: rows must not be negative; N, K and experts must be positive", name);
   if (x->K % 32) return fail(NVFP4_ERR_SHAPE, "%s: K=%d must be a multiple of 32", name, x->K);
   if (x->experts > kMaxExpertsApi) return fail(NVFP4_ERR_SHAPE, "%s: %d experts, at most %d", name, x->experts, kMaxExpertsApi);
   if (x->experts != 1 && !x->offsets) return fail(NVFP4_ERR_NULL, "%s: several experts need offsets", name);
-  if (x->ldc < x->N) return fail(NVFP4_ERR_SHAPE, "%s: ldc=%lld < N=%d", name, (long long)x->ldc, x->N);
+  if (!codes && x->ldc < x->N)
+    return fail(NVFP4_ERR_SHAPE, "%s: ldc=%lld < N=%d", name, (long long)x->ldc, x->N);
+  if (codes && (x->N % 32 || !x->b2))
+    return fail(NVFP4_ERR_SHAPE, "%s: an MXFP4 result is for two products, N=%d a multiple of 32", name, x->N);
   if (x->K > (1 << 24) || (static_cast<int64_t>(x->rows) / 32 + x->experts) * ((static_cast<int64_t>(x->N) + 63) / 64) >
                                INT32_MAX)
     return fail(NVFP4_ERR_SHAPE, "%s: too large", name);
   if (x->rows == 0) return NVFP4_OK;
-  if (!x->a || !x->b || !x->sfa || !x->sfb || !x->c || !x->b2 != !x->sfb2)
+  if (!x->a || !x->b || !x->sfa || !x->sfb || !x->c || !x->b2 != !x->sfb2 || (codes && !x->c_scales))
     return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
   if (!aligned(x->a, 16) || !aligned(x->b, 16) || !aligned(x->b2, 16) || !aligned(x->sfa, 16) || !aligned(x->sfb, 16) ||
-      !aligned(x->sfb2, 16) || !aligned(x->c, dtype_size(x->out_dtype)) || !aligned(x->offsets, 4))
+      !aligned(x->sfb2, 16) || !aligned(x->c, codes ? 16 : dtype_size(x->out_dtype)) || !aligned(x->c_scales, 16) || !aligned(x->offsets, 4))
     return fail(NVFP4_ERR_ALIGN, "%s: codes and scales need 16-byte alignment, c that of its type", name);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "%s: no CUDA device", name);
-  MxGemmArgs g{x->a,    x->b, x->b2, x->sfa,     x->sfb,       x->sfb2, x->c,            x->offsets,
+  MxGemmArgs g{x->a,    x->b, x->b2, x->sfa,     x->sfb,       x->sfb2, x->c, x->c_scales, x->offsets,
                x->rows, x->N, x->K,  x->experts, x->out_dtype, x->ldc,  status_ptr(dev), read_env_options().fault_inject};
   const char* why = nullptr;
   const cudaError_t e = launch_mx_gemm(g, num_sms_of(dev), static_cast<cudaStream_t>(x->stream), &why);

@@ -162,6 +162,7 @@ cudaError_t launch_mx_dequantize(const MxQuantArgs& a, int num_sms, cudaStream_t
 struct MxGemmArgs {
   const void *a, *b, *b2, *sfa, *sfb, *sfb2;  // b2 null: not gated
   void* c;
+  void* c_scales;      // out_dtype 3 (MXFP4, gated): the scales of c's codes
   const int* offsets;  // rows sorted by expert (or null: one weight matrix)
   int rows, N, K, experts, out_dtype;
   int64_t ldc;

@@ -2,7 +2,7 @@
 // tokens, of one weight matrix or of one per expert:
 //
 //   y[r, n] = sum_k (a sa)[r, k] (b[e(r)] sb[e(r)])[n, k]               r: rows sorted by expert
-//   gated:    silu(a . b1^T) * (a . b2^T)
+//   gated:    silu(a . b1^T) * (a . b2^T), which may leave as MXFP4
 //
 // fp32 sums in the tensor cores, rounded once to the output's type.
 //
@@ -53,6 +53,7 @@
 #include "common.cuh"
 #include "experts.cuh"
 #include "kernels.h"
+#include "mx.cuh"
 
 namespace nvfp4 {
 
@@ -80,6 +81,7 @@ struct Params {
   const uint8_t* sfw2;  // of b2 (gated)
   const uint8_t* sfx;   // scales of the tokens
   void* c;
+  uint8_t* c_scales;   // Codes: the result's scales (c: its codes)
   const int* offsets;  // null: one expert with all rows
   int rows, N, K, experts;
   int64_t ldc;
@@ -95,6 +97,11 @@ struct Params {
   int tma;        // TMA stores of C
   int* status;
   int inject;     // test hook: CTA 0 withholds its first weight load
+};
+
+// The type of a result that is quantised to MXFP4 on its way out.
+struct Codes {
+  uint8_t pair;
 };
 
 // How CTAs share the tiles: one each; K split over a cluster; two CTAs a tile.
@@ -319,11 +326,9 @@ __device__ __forceinline__ int staged(int t, int f) {
   const int b = f * static_cast<int>(sizeof(OutT));
   return (b >> 7) * (kChunk * 128) + t * 128 + ((b & 112) ^ ((t & 7) << 4)) + (b & 15);
 }
-// Staging buffers per group: 16-bit types write one while the other is stored.
-template <typename OutT>
-__host__ __device__ constexpr int staging_bufs() {
-  return sizeof(OutT) == 2 ? 2 : 1;
-}
+// Staging buffers per group: 32-bit types have one, the others write one while
+// the other is stored.
+__host__ __device__ constexpr int staging_bufs(size_t out_size) { return out_size <= 2 ? 2 : 1; }
 
 // kSplitK: groups of 8 tokens that a rank adds up, and its space for the others'
 // partial sums of them: 128 rows x 8 tokens in fp32 per group and rank.
@@ -346,7 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int x_rows = kPair ? p.tn / 2 : p.tn;  // token rows of a stage
   const int stage_bytes = kABytes + x_rows * kBKBytes;
   const int sf_bytes = (kSfW + p.nblk) * kSfBytes;
-  constexpr int kBufs = staging_bufs<OutT>(), kStaged = kChunk * kF * sizeof(OutT);
+  constexpr bool kCodes = std::is_same<OutT, Codes>::value;
+  static_assert(!kCodes || kGate, "only gated results are quantised");
+  constexpr int kBufs = staging_bufs(sizeof(OutT)), kStaged = kChunk * kF * sizeof(OutT);
   uint8_t* staging = smem + S * stage_bytes;  // per group kBufs of kStaged bytes (1024-aligned)
   uint8_t* sums = staging + kGroups * kBufs * kStaged;  // kSplit: the other ranks' partial sums
   uint8_t* sfbuf = sums + (kSplit ? sums_bytes(p.tn, p.splits) : 0);
@@ -436,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int t0 = kSplit ? blockIdx.x / p.splits : kPair ? blockIdx.x >> 1 : blockIdx.x;
   const int step = kSplit ? total : kPair ? gridDim.x >> 1 : gridDim.x;  // kSplit: one tile per cluster
   const int rank = kMode == kWhole ? 0 : static_cast<int>(cluster_ctarank());
+  // A tile's first scale row, of its tokens and of a quantised result.
+  auto scale0 = [&](const Tile& o) { return static_cast<int64_t>(o.blk) * 128 + o.in_blk; };
   // First feature of this CTA's weight rows.
   auto feature0 = [&](const Tile& o) { return kPair ? (2 * o.ft + rank) * kF : o.ft * kF; };
   const int k0 = kSplit ? rank * KT / p.splits : 0, k1 = kSplit ? (rank + 1) * KT / p.splits : KT;
@@ -714,9 +723,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   // transposed by stmatrix so that a token's features lie together, and leave in
   // 16-byte stores.
   int buf = 0;
-  auto emit = [&](auto width, uint32_t* r, int64_t row0, int f0, int valid) {
+  auto emit = [&](auto width, uint32_t* r, int64_t row0, int64_t scale_row, int f0, int valid) {
     constexpr int G = decltype(width)::value, kR = 4 * G;
-    constexpr int kHalves = kGate && G == 1 ? 1 : 2;       // row halves that this warp computes
+    constexpr bool kOne = kCodes && G == 1;  // the warps of x1 compute all: a block needs its 32 features in a warp
+    [[maybe_unused]] constexpr int kHalves = kGate && G == 1 && !kOne ? 1 : 2;  // row halves that this warp computes
     constexpr int kTok = kGate && G > 1 ? G / 2 : G;       // its groups of 8 tokens
     uint8_t* out = staging + (group * kBufs + buf) * kStaged;
     if (kBufs == 2) {
@@ -726,7 +736,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_sync(1 + group, 128);
     }
     int feature = q * 32, token = 0;  // of what this warp computes
-    if (kGate) {
+    if (kOne) {
+      uint4* const box = exch + group * 512 + (q & 1) * 256 + lane;
+      if (q >= 2) {
+        box[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        box[32] = make_uint4(r[4], r[5], r[6], r[7]);
+      }
+      bar_sync(3 + group * 2 + (q & 1), 64);
+      if (q < 2) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const uint4 o = box[32 * v];
+          const uint32_t other[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            r[4 * v + i] = __float_as_uint(silu_mul(__uint_as_float(r[4 * v + i]), __uint_as_float(other[i])));
+        }
+      }
+    } else if (kGate) {
       // Warps 0 and 1 of a group hold x1, 2 and 3 x2 of the same outputs: each
       // gives its partner half of its values (half of the tokens, or of 8 tokens
       // half of the rows) and computes the other half.
@@ -764,7 +791,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       token = G > 1 && !first ? 8 * kTok : 0;
     }
     // r[half][4 kTok] now, kHalves halves.
-    if constexpr (sizeof(OutT) == 2) {
+    if constexpr (kCodes) {
+      // A token's 32 features of this warp are a block: four in each of the eight
+      // lanes with its columns (lane / 4 + 8 m), so the largest comes by three
+      // shuffles; a lane and its neighbour put their nibbles together, and the
+      // bytes meet in shared memory: per token 2 x 16 bytes of codes, then scales.
+      if (!kOne || q < 2) {
+        const int f = lane >> 2;
+#pragma unroll
+        for (int j = 0; j < kTok; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v[4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[k] = __uint_as_float(r[(k >> 1) * 4 * kTok + 4 * j + 2 * (k & 1) + i]);
+              top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const uint32_t code = scale_code(top);
+            const float inv = inverse_scale(code);
+            const uint32_t n = code == 255u ? 0u : e2m1_pair(v[0] * inv, v[1] * inv) | e2m1_pair(v[2] * inv, v[3] * inv) << 8;
+            uint32_t bytes = (n & 0xfu) | (n & 0xf0u) << 4 | (n & 0xf00u) << 8 | (n & 0xf000u) << 12;
+            bytes <<= 4 * (f & 1);
+            bytes |= __shfl_xor_sync(0xffffffffu, bytes, 4);
+            const int tok = token + 8 * j + 2 * (lane & 3) + i;
+            uint8_t* const at = out + tok * 32 + (q & 1) * 16 + (f >> 1);
+            if ((f & 1) == 0) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) at[4 * k] = static_cast<uint8_t>(bytes >> (8 * k));
+            }
+            if (f == 0) out[kChunk * 32 + tok * 2 + (q & 1)] = static_cast<uint8_t>(code);
+          }
+      }
+    } else if constexpr (sizeof(OutT) == 2) {
 #pragma unroll
       for (int j = 0; j < kTok; ++j) {
         uint32_t m[2 * kHalves];
@@ -792,7 +854,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tma) fence_proxy_async_smem();
     if (kBufs == 2 && gtid == 0) bulk_wait_group_read0();  // the other buffer, which the next step writes, is read
     bar_sync(1 + group, 128);
-    if (tma) {
+    if constexpr (kCodes) {
+      const int tok = (gtid & 63) >> 1, f = f0 + 32 * (gtid & 1);  // f: of the block
+      if (tok < valid && f < p.N) {
+        if (gtid < 64)
+          *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c) + (row0 + tok) * (p.N >> 1) + (f >> 1)) =
+              *reinterpret_cast<const uint4*>(out + tok * 32 + (gtid & 1) * 16);
+        else
+          p.c_scales[mx_scale_word(scale_row + tok, f >> 7, (p.N + 127) >> 7) + ((f >> 5) & 3)] =
+              out[kChunk * 32 + tok * 2 + (gtid & 1)];
+      }
+    } else if (tma) {
       if (gtid == 0) {
 #pragma unroll
         for (int b = 0; b < kStaged / (kChunk * 128); ++b)
@@ -850,17 +922,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_16x256b_x4(tacc + (16u << 16) + c0, r + 16);
         tmem_wait_ld();
         if (c0 + kGroups * kChunk >= o.rows) release();
-        emit(std::integral_constant<int, 4>(), r, o.row0 + c0, feature0(o), min(kChunk, o.rows - c0));
+        emit(std::integral_constant<int, 4>(), r, o.row0 + c0, scale0(o) + c0, feature0(o), min(kChunk, o.rows - c0));
       }
       if (++acc == p.acc_bufs) {
         acc = 0;
         acc_phase ^= 1;
       }
     }
-    // Rows that belong to no expert.
-    if (group == 0)
-      for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
-        for (int f = gtid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
+    // Rows that belong to no expert (their codes stay as they were).
+    if constexpr (!kCodes) {
+      if (group == 0)
+        for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
+          for (int f = gtid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
+    }
   }
 
   if (kSplit) {
@@ -930,7 +1004,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             r[4 * h + 2] = __float_as_uint(__uint_as_float(r[4 * h + 2]) + v.z);
             r[4 * h + 3] = __float_as_uint(__uint_as_float(r[4 * h + 3]) + v.w);
           }
-        emit(std::integral_constant<int, 1>(), r, o.row0 + 8 * g, feature0(o), min(8, o.rows - 8 * g));
+        emit(std::integral_constant<int, 1>(), r, o.row0 + 8 * g, scale0(o) + 8 * g, feature0(o), min(8, o.rows - 8 * g));
       }
     }
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
@@ -955,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 size_t fixed_smem(int out_size, bool gate, int experts) {
-  const int staged = kChunk * (gate ? 64 : 128) * out_size * (out_size == 2 ? 2 : 1);
+  const int staged = kChunk * (gate ? 64 : 128) * out_size * staging_bufs(out_size);
   return 1024 /* alignment */ + kGroups * (staged + (gate ? 512 * 16 : 0)) + (3 * kMaxStages + 6) * 8 + 8 +
          3 * (static_cast<size_t>(experts) + 1) * 4;
 }
@@ -987,17 +1061,19 @@ cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, 
                     txs, p.tma ? tc : tx, p);
 }
 
+template <typename OutT, bool kGate>
+cudaError_t launch_mode(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream,
+                        const char** why) {
+  return p.splits > 1 ? launch<OutT, kGate, kSplitK>(g, p, smem, grid, stream, why)
+         : p.pair     ? launch<OutT, kGate, kPairs>(g, p, smem, grid, stream, why)
+                      : launch<OutT, kGate, kWhole>(g, p, smem, grid, stream, why);
+}
+
 template <typename OutT>
 cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int grid, cudaStream_t stream,
                        const char** why) {
-  if (p.splits > 1)
-    return g.b2 ? launch<OutT, true, kSplitK>(g, p, smem, grid, stream, why)
-                : launch<OutT, false, kSplitK>(g, p, smem, grid, stream, why);
-  if (p.pair)
-    return g.b2 ? launch<OutT, true, kPairs>(g, p, smem, grid, stream, why)
-                : launch<OutT, false, kPairs>(g, p, smem, grid, stream, why);
-  return g.b2 ? launch<OutT, true, kWhole>(g, p, smem, grid, stream, why)
-              : launch<OutT, false, kWhole>(g, p, smem, grid, stream, why);
+  return g.b2 ? launch_mode<OutT, true>(g, p, smem, grid, stream, why)
+              : launch_mode<OutT, false>(g, p, smem, grid, stream, why);
 }
 
 // Tile shapes and what a K tile of theirs takes, in us, when every SM has one:
@@ -1060,12 +1136,13 @@ Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms
 
 cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why) {
   const bool gate = g.b2 != nullptr;
-  const int out_size = g.out_dtype == 2 ? 4 : 2;
+  const int out_size = g.out_dtype == 2 ? 4 : g.out_dtype == 3 ? 1 : 2;
   Params p{};
   p.sfw = static_cast<const uint8_t*>(g.sfb);
   p.sfw2 = static_cast<const uint8_t*>(g.sfb2);
   p.sfx = static_cast<const uint8_t*>(g.sfa);
   p.c = g.c;
+  p.c_scales = static_cast<uint8_t*>(g.c_scales);
   p.offsets = g.offsets;
   p.rows = g.rows;
   p.N = g.N;
@@ -1074,7 +1151,7 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.ldc = g.ldc;
   p.status = g.status;
   p.inject = g.inject;
-  p.vec = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
+  p.vec = g.out_dtype != 3 && reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
   // (A TMA store ends its rows at multiples of 16 bytes only.)
   p.tma = p.vec && static_cast<int64_t>(g.N) * out_size % 16 == 0;
   const int KT = (g.K + kBK - 1) / kBK;
@@ -1106,6 +1183,7 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const size_t smem = fixed + p.stages * stage;
   return g.out_dtype == 0   ? launch_out<__half>(g, p, smem, static_cast<int>(grid), stream, why)
          : g.out_dtype == 1 ? launch_out<__nv_bfloat16>(g, p, smem, static_cast<int>(grid), stream, why)
+         : g.out_dtype == 3 ? launch_mode<Codes, true>(g, p, smem, static_cast<int>(grid), stream, why)
                             : launch_out<float>(g, p, smem, static_cast<int>(grid), stream, why);
 }
 

@@ -73,8 +73,8 @@ class MxQuantArgs(ctypes.Structure):
 
 class MxGemmArgs(ctypes.Structure):
     """nvfp4_mx_gemm_args of include/nvfp4_b200.h."""
-    _fields_ = [("a", _P), ("b", _P), ("b2", _P), ("sfa", _P), ("sfb", _P), ("sfb2", _P), ("c", _P), ("offsets", _P),
-                ("rows", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("experts", ctypes.c_int32),
+    _fields_ = [("a", _P), ("b", _P), ("b2", _P), ("sfa", _P), ("sfb", _P), ("sfb2", _P), ("c", _P),
+                ("c_scales", _P), ("offsets", _P), ("rows", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("experts", ctypes.c_int32),
                 ("out_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("ldc", _L), ("stream", _P)]
 
 
@@ -104,7 +104,7 @@ def _packer(layout: str):
 # The last three structs as bytes in one call, for calls of a few microseconds: filling a ctypes.Structure of as many
 # fields takes four times as long.  A null pointer is 0.
 pack_mx_quant = _packer("@5P6i2qP")
-pack_mx_gemm = _packer("@8P6iqP")
+pack_mx_gemm = _packer("@9P6iqP")
 pack_moe = _packer("@7P6i2qP")
 
 

@@ -206,12 +206,12 @@ def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, dow
     """The experts' MLP on x [T, H]: y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].
 
     gate, up: operands (packed, scales) of [experts, N, H] weights, down of [experts, H, N], as mx.quantize makes them
-    (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  The tokens and the gated values are
-    quantised to MXFP4 on the way; x and the result are fp16, bf16 or fp32, and so are the values between the
-    products.  Six launches (seven for more than 32768 slots), no synchronisation."""
+    (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  x and the result are fp16, bf16 or
+    fp32; the tokens are quantised to MXFP4 as they are sorted, the gated values in the product's epilogue, and the
+    down projection's rows have x's type.  Five launches (six for more than 32768 slots), no synchronisation."""
     if gate[0].dim() != 3:
         _fail(f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
     routing = sort(ids, gate[0].shape[0])
-    h = mx.dual_gemm(*quantize_tokens(x, routing), *gate, *up, offsets=routing.offsets, out_dtype=x.dtype)
-    y = mx.gemm(*mx.quantize(h, offsets=routing.offsets), *down, offsets=routing.offsets, out_dtype=x.dtype)
-    return combine(y, weights, routing)
+    offsets = routing.offsets
+    h = mx.dual_gemm(*quantize_tokens(x, routing), *gate, *up, offsets=offsets, quantize=True)
+    return combine(mx.gemm(*h, *down, offsets=offsets, out_dtype=x.dtype), weights, routing)

@@ -178,8 +178,8 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor
     return out
 
 
-def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype):
-    code = _DTYPES.get(out_dtype)
+def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype, quantize=False):
+    code = 3 if quantize else _DTYPES.get(out_dtype)
     if code is None:
         _fail(f"{who}: out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
     experts, dim = None, 2
@@ -195,18 +195,24 @@ def _product(who, a, sa, b1, s1, b2, s2, offsets, out_dtype):
         _fail(f"{who}: weights {tuple(b2.shape)} do not fit weights {tuple(shape)}")
     dev = _device(who, a, sa, b1, s1, b2, s2, offsets)
     n = shape[-2]
-    c = a.new_empty((rows, n), dtype=out_dtype)
+    if quantize:
+        if n == 0 or n % 32:
+            _fail(f"{who}: N={n} must be a positive multiple of 32 for a quantised result")
+        c = a.new_empty((rows, n // 2), dtype=FP4X2)
+        sc = a.new_empty((scale_blocks(rows, experts), -(-n // 128), 32, 4, 4), dtype=E8M0)
+    else:
+        c, sc = a.new_empty((rows, n), dtype=out_dtype), None
     if rows and n:
         gated = b2 is not None
         rc = _lib.load().nvfp4_mx_gemm(_lib.pack_mx_gemm(
             a.data_ptr(), b1.data_ptr(), b2.data_ptr() if gated else 0, sa.data_ptr(), s1.data_ptr(),
-            s2.data_ptr() if gated else 0, c.data_ptr(), 0 if offsets is None else offsets.data_ptr(), rows, n,
-            2 * k2, experts or 1, code, 0, n, _raw_stream(dev)))
+            s2.data_ptr() if gated else 0, c.data_ptr(), sc.data_ptr() if quantize else 0,
+            0 if offsets is None else offsets.data_ptr(), rows, n, 2 * k2, experts or 1, code, 0, n, _raw_stream(dev)))
         if rc:
             _lib.check(rc)
         if _CHECK_STATUS:
             _post()
-    return c
+    return (c, sc) if quantize else c
 
 
 def gemm(a, sa, b, sb, offsets: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -217,7 +223,10 @@ def gemm(a, sa, b, sb, offsets: torch.Tensor | None = None, out_dtype: torch.dty
     return _product("mx.gemm", a, sa, b, sb, None, None, offsets, out_dtype)
 
 
-def dual_gemm(a, sa, b1, sb1, b2, sb2, offsets: torch.Tensor | None = None,
-              out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """silu(a . b1^T) * (a . b2^T), otherwise as gemm; both products stay in fp32."""
-    return _product("mx.dual_gemm", a, sa, b1, sb1, b2, sb2, offsets, out_dtype)
+def dual_gemm(a, sa, b1, sb1, b2, sb2, offsets: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+              quantize: bool = False):
+    """silu(a . b1^T) * (a . b2^T), otherwise as gemm; both products stay in fp32.
+
+    quantize=True (N % 32 == 0): the result as an MXFP4 operand (packed, scales), quantised from fp32 in the product's
+    epilogue: what mx.quantize of the fp32 result, with the same offsets, gives."""
+    return _product("mx.dual_gemm", a, sa, b1, sb1, b2, sb2, offsets, out_dtype, quantize)

@@ -69,6 +69,7 @@ def test_refusals():
             (lambda: mx.gemm(a, sa, b, sb, offsets=off), "2 experts"),
             (lambda: mx.gemm(a, sa, b.view(1, 8, 32), sb.view(1, 1, 1, 32, 4, 4)), "2 dimensions"),
             (lambda: mx.dual_gemm(a, sa, b, sb, b[:4], sb), "do not fit"),
+            (lambda: mx.dual_gemm(*((torch.zeros((8, 32), dtype=torch.uint8), sb) * 3), quantize=True), "CUDA|N=8"),
             (lambda: mx.gemm(a, sa, b.view(2, 4, 32), sb.expand(2, 1, 1, 32, 4, 4).contiguous(), offsets=off),
              "scales")]:
         with pytest.raises(_lib.Nvfp4Error, match=what):
@@ -83,7 +84,10 @@ def test_c_refusals():
         return lib.nvfp4_mx_gemm(ctypes.byref(_lib.MxGemmArgs(**{**d, **kw})))
 
     assert lib.nvfp4_mx_gemm(None) == 3
-    assert rc(out_dtype=3) == 1 and rc(rows=-1) == 1 and rc(N=0) == 1 and rc(K=48) == 1 and rc(K=0) == 1
+    assert rc(out_dtype=4) == 1 and rc(out_dtype=3) == 1 and rc(rows=-1) == 1
+    codes = dict(out_dtype=3, b2=fake, sfb2=fake)
+    assert rc(**codes) == 1 and rc(**codes, N=32) == 3 and rc(**codes, N=32, c_scales=fake + 8) == 2
+    assert rc(**codes, N=32, c_scales=fake, c=fake + 8) == 2 and rc(N=0) == 1 and rc(K=48) == 1 and rc(K=0) == 1
     assert rc(experts=0) == 1 and rc(experts=1025, offsets=fake) == 1 and rc(ldc=7) == 1
     assert rc(rows=2 ** 31 - 1, N=2 ** 31 - 1, ldc=2 ** 31) == 1 and rc(K=1 << 25) == 1
     assert rc(experts=2) == 3 and rc(a=None) == 3 and rc(b2=fake) == 3 and rc(sfb2=fake) == 3
@@ -113,7 +117,7 @@ def test_struct_layout_matches_header(tmp_path):
 
 
 def test_packed_bytes_equal_the_structs():
-    for py, pack, n in [(_lib.MxQuantArgs, _lib.pack_mx_quant, 14), (_lib.MxGemmArgs, _lib.pack_mx_gemm, 16),
+    for py, pack, n in [(_lib.MxQuantArgs, _lib.pack_mx_quant, 14), (_lib.MxGemmArgs, _lib.pack_mx_gemm, 17),
                         (_lib.MoeArgs, _lib.pack_moe, 16)]:
         values = [3 * i + 1 for i in range(n)]
         assert bytes(py(*values)) == pack(*values)
@@ -265,6 +269,48 @@ def test_experts(dtype, counts, tail, n, k):
     assert _lib.device_status(True) == 0
 
 
+def same_operand(got, want, rows, at):
+    """Two operands' codes and scales of the rows that an expert has."""
+    used = len(at)
+    assert got[0].dtype == torch.float4_e2m1fn_x2 and got[0].shape == want[0].shape and got[1].shape == want[1].shape
+    assert torch.equal(got[0].view(torch.uint8)[:used], want[0].view(torch.uint8)[:used])
+    n = 2 * got[0].shape[1]
+    a, b = (mxref.plain_scales(o[1].view(torch.uint8).cpu().numpy(), used, n, at) for o in (got, want))
+    np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 32, 64), (5, 96, 160), (33, 160, 96), (200, 96, 288), (17, 320, 4096),
+                                   (1, 64, 16384), (70, 128, 8192), (128, 160, 16384), (250, 2048, 64), (600, 1856, 64),
+                                   (400, 2048, 96), (600, 2048, 320), (1013, 2048, 544), (3000, 1056, 32)])
+def test_quantized_result(m, n, k):
+    """The codes and scales that mx.quantize gives for the fp32 result, on every tile shape and K split."""
+    g = np.random.RandomState(m + n + k)
+    low = 127 - int(np.log2(k) / 2) - 4
+    a, b1, b2 = operand(m, k, g, low, low + 3), operand(n, k, g), operand(n, k, g)
+    a[0][0] = 0  # a zero row: zero blocks
+    if m > 4:
+        a[1][3, 0] = 255  # a NaN row
+        b1[1][40 % n, k // 32 - 1] = 255  # a NaN column: its block in every row
+    ops = on_gpu(*a) + on_gpu(*b1) + on_gpu(*b2)
+    same_operand(mx.dual_gemm(*ops, quantize=True), mx.quantize(mx.dual_gemm(*ops, out_dtype=torch.float32)), m,
+                 np.arange(m))
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k", [(96, 288), (128, 512), (2048, 96)])
+@pytest.mark.parametrize("counts,tail", [c for c in GROUPS if len(c[0]) < 100])
+def test_quantized_result_of_experts(counts, tail, n, k):
+    if n == 2048 and len(counts) > 6:
+        n = 320
+    a, (b1, b2), offsets, _ = grouped(counts, tail, n, k, 5, both=True)
+    at, _ = mxref.scale_rows(offsets.tolist())
+    want = mx.quantize(mx.dual_gemm(*a, *b1, *b2, offsets=offsets, out_dtype=torch.float32), offsets=offsets)
+    same_operand(mx.dual_gemm(*a, *b1, *b2, offsets=offsets, quantize=True), want, sum(counts) + tail, at)
+    assert _lib.device_status(True) == 0
+
+
 @pytest.mark.gpu
 def test_offsets_that_fall_or_leave_the_rows_stay_in_bounds():
     g = np.random.RandomState(8)
@@ -349,7 +395,7 @@ def test_rows_of_c_apart(m, n, k, ldc, shift):
     (pa, sa), (pb, sb) = on_gpu(*a), on_gpu(*b)
     c = torch.full((m + 1, ldc), 7.0, dtype=torch.bfloat16, device="cuda")
     args = _lib.MxGemmArgs(pa.data_ptr(), pb.data_ptr(), None, sa.data_ptr(), sb.data_ptr(), None,
-                           c.data_ptr() + 2 * shift, None, m, n, k, 1, 1, 0, ldc,
+                           c.data_ptr() + 2 * shift, None, None, m, n, k, 1, 1, 0, ldc,
                            torch.cuda.current_stream().cuda_stream)
     _lib.check(_lib.load().nvfp4_mx_gemm(ctypes.byref(args)))
     flat = c.reshape(-1)[shift:shift + m * ldc].view(m, ldc)

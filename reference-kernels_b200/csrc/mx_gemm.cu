@@ -792,39 +792,55 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // r[half][4 kTok] now, kHalves halves.
     if constexpr (kCodes) {
-      // A token's 32 features of this warp are a block: four in each of the eight
-      // lanes with its columns (lane / 4 + 8 m), so the largest comes by three
-      // shuffles; a lane and its neighbour put their nibbles together, and the
-      // bytes meet in shared memory: per token 2 x 16 bytes of codes, then scales.
+      // A token's 32 features of this warp are a block, four in each of the eight
+      // lanes with its columns (lane / 4 + 8 k).  The scale needs only the largest
+      // exponent: those of the lane's 2 kTok tokens go through three shuffles
+      // together, a byte each.  Codes of neighbouring features lie in neighbouring
+      // lanes (lane ^ 4), which give each other half of the tokens, so that one
+      // shuffle brings whole bytes together.  They meet in shared memory: per token
+      // 2 x 16 bytes of codes, then the scales.
       if (!kOne || q < 2) {
+        constexpr int kT = 2 * kTok;
         const int f = lane >> 2;
+        const bool odd = f & 1;
+        auto value = [&](int t, int k) {
+          return __uint_as_float(r[(k >> 1) * 4 * kTok + 4 * (t >> 1) + 2 * (k & 1) + (t & 1)]);
+        };
+        uint32_t exponents = 0;
 #pragma unroll
-        for (int j = 0; j < kTok; ++j)
+        for (int t = 0; t < kT; ++t) {
+          uint32_t top = 0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float v[4];
-            uint32_t top = 0;
+          for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(value(t, k)) & 0x7fffffffu);
+          exponents |= (top >> 23) << (8 * t);
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[k] = __uint_as_float(r[(k >> 1) * 4 * kTok + 4 * j + 2 * (k & 1) + i]);
-              top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-            }
+        for (int d = 4; d < 32; d <<= 1) exponents = __vmaxu4(exponents, __shfl_xor_sync(0xffffffffu, exponents, d));
+        uint32_t half[2] = {0, 0};  // 16 bits of codes per token
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const uint32_t code = scale_code(top);
-            const float inv = inverse_scale(code);
-            const uint32_t n = code == 255u ? 0u : e2m1_pair(v[0] * inv, v[1] * inv) | e2m1_pair(v[2] * inv, v[3] * inv) << 8;
-            uint32_t bytes = (n & 0xfu) | (n & 0xf0u) << 4 | (n & 0xf00u) << 8 | (n & 0xf000u) << 12;
-            bytes <<= 4 * (f & 1);
-            bytes |= __shfl_xor_sync(0xffffffffu, bytes, 4);
-            const int tok = token + 8 * j + 2 * (lane & 3) + i;
-            uint8_t* const at = out + tok * 32 + (q & 1) * 16 + (f >> 1);
-            if ((f & 1) == 0) {
+        for (int t = 0; t < kT; ++t) {
+          const uint32_t code = scale_code((exponents >> (8 * t) & 255u) << 23);
+          const float inv = inverse_scale(code);
+          const uint32_t n = e2m1_pair(value(t, 0) * inv, value(t, 1) * inv) |
+                             e2m1_pair(value(t, 2) * inv, value(t, 3) * inv) << 8;
+          half[t / kTok] |= (code == 255u ? 0u : n) << (16 * (t % kTok));
+          if (f == 0)
+            out[kChunk * 32 + (token + 8 * (t >> 1) + 2 * lane + (t & 1)) * 2 + (q & 1)] = static_cast<uint8_t>(code);
+        }
+        const uint32_t mine = odd ? half[1] : half[0];
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? half[0] : half[1], 4);
+        auto spread = [](uint32_t x) {
+          return (x & 0xfu) | (x & 0xf0u) << 4 | (x & 0xf00u) << 8 | (x & 0xf000u) << 12;
+        };
 #pragma unroll
-              for (int k = 0; k < 4; ++k) at[4 * k] = static_cast<uint8_t>(bytes >> (8 * k));
-            }
-            if (f == 0) out[kChunk * 32 + tok * 2 + (q & 1)] = static_cast<uint8_t>(code);
-          }
+        for (int u = 0; u < kTok; ++u) {
+          const uint32_t x = spread(mine >> (16 * u)), y = spread(other >> (16 * u));
+          const uint32_t bytes = odd ? y | x << 4 : x | y << 4;
+          const int t = u + (odd ? kTok : 0), tok = token + 8 * (t >> 1) + 2 * (lane & 3) + (t & 1);
+          uint8_t* const at = out + tok * 32 + (q & 1) * 16 + (f >> 1);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) at[4 * k] = static_cast<uint8_t>(bytes >> (8 * k));
+        }
       }
     } else if constexpr (sizeof(OutT) == 2) {
 #pragma unroll

@@ -28,12 +28,12 @@
 // own half of them and of the tokens, which halves the token bytes per SM.
 //
 // What bounds it, on B200: few tokens by HBM -- 32 tokens over 64 experts, gated,
-// 2048x4096: 77 us for 0.56 GB, 7.3 TB/s, above the 6.6 TB/s of a copy; one token
-// through 7168x16384 15.4 us, 9.5 of them traffic, the rest set-up, the first
+// 2048x4096: 76 us for 0.56 GB, 7.4 TB/s, above the 6.6 TB/s of a copy; one token
+// through 7168x16384 15.2 us, 9.5 of them traffic, the rest set-up, the first
 // loads' latency and the exchange of partial sums.  Many tokens by what an SM
 // takes from L2: a pair's 192-token tile needs 31 KB per 384 cycles of MMA, and
-// 57 bytes a clock arrive of the 64 that an SM's port has -- 1000x7168x16384 48 us
-// (4.9 PFLOP/s), 8192x7168x4096 98 us, 8192x7168x16384 329 us (5.85 PFLOP/s, 0.87
+// 57 bytes a clock arrive of the 64 that an SM's port has -- 1000x7168x16384 47 us
+// (5.0 PFLOP/s), 8192x7168x4096 93 us, 8192x7168x16384 327 us (5.9 PFLOP/s, 0.88
 // of 4 x the measured bf16 rate).  Over seconds the power cap takes 15 % of that.
 // The offsets are read on the device: every CTA builds the table of the experts'
 // rows, scale blocks and tiles in shared memory and walks the same tile list, so

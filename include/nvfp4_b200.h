@@ -205,7 +205,7 @@ int nvfp4_dual_gemm_call(const nvfp4_gemm_args* args);
  * min(rows, experts) + rows/128 blocks hold them whatever the offsets.  Rows
  * behind offsets[experts] belong to nobody: what reads rows skips them, what
  * writes rows of values writes zeros there, and the quantiser leaves them as
- * they were.  At most 1024 experts. */
+ * they were.  At most 1024 experts; rows, K, N, hidden and slots below 2^31 - 2^20. */
 
 /* x (fp16, bf16 or fp32: dtype 0, 1, 2) and its MXFP4 form.  x has `experts`
  * matrices of `rows` rows of K elements (x_estride, x_rstride elements apart),

@@ -418,6 +418,9 @@ NVFP4_API int nvfp4_scales_from_blocked(const void* blk, void* plain, int rows, 
 
 // ------------------------------------------------------------------ MXFP4 and experts
 constexpr int kMaxExpertsApi = 1024;
+// Sizes of one dimension: the kernels round them up and step past them in 32-bit
+// integers, by less than 2^20.
+constexpr int64_t kMaxSize = INT32_MAX - (1 << 20);
 
 static int64_t dtype_size(int dtype) { return dtype == 2 ? 4 : 2; }
 
@@ -438,8 +441,9 @@ static int mx_quant_args(const char* name, const nvfp4_mx_quant_args* x, bool qu
   const int64_t rows = x->offsets ? x->rows : static_cast<int64_t>(x->rows) * x->experts;
   const int64_t units = rows * ((static_cast<int64_t>(x->K) + 127) / 128 * 4);  // scales, padding included
   const int64_t sorted = x->slots ? static_cast<int64_t>(x->rows) * x->top : rows;
-  if (rows > INT32_MAX || units > INT32_MAX || sorted > INT32_MAX || (x->columns && x->rows > 65535 * 256))
-    return fail(NVFP4_ERR_SHAPE, "%s: too many rows", name);
+  if (rows > kMaxSize || x->K > kMaxSize || units > kMaxSize || sorted > kMaxSize ||
+      (x->columns && x->rows > 65535 * 256))
+    return fail(NVFP4_ERR_SHAPE, "%s: too large", name);
   if (rows > 0 && sorted > 0) {
     if (!x->x || !x->packed || !x->scales) return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
     if (!aligned(x->x, quantize ? dtype_size(x->dtype) : 32) || !aligned(x->packed, 16) || !aligned(x->scales, 16) ||
@@ -491,8 +495,8 @@ NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
     return fail(NVFP4_ERR_SHAPE, "%s: ldc=%lld < N=%d", name, (long long)x->ldc, x->N);
   if (codes && (x->N % 32 || !x->b2))
     return fail(NVFP4_ERR_SHAPE, "%s: an MXFP4 result is for two products, N=%d a multiple of 32", name, x->N);
-  if (x->K > (1 << 24) || (static_cast<int64_t>(x->rows) / 32 + x->experts) * ((static_cast<int64_t>(x->N) + 63) / 64) >
-                               INT32_MAX)
+  if (x->rows > kMaxSize || x->N > kMaxSize || x->K > (1 << 24) ||
+      (static_cast<int64_t>(x->rows) / 32 + x->experts) * ((static_cast<int64_t>(x->N) + 63) / 64) > kMaxSize)
     return fail(NVFP4_ERR_SHAPE, "%s: too large", name);
   if (x->rows == 0) return NVFP4_OK;
   if (!x->a || !x->b || !x->sfa || !x->sfb || !x->c || !x->b2 != !x->sfb2 || (codes && !x->c_scales))
@@ -512,14 +516,14 @@ NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
 
 NVFP4_API int64_t nvfp4_moe_sort_workspace(int n, int experts) {
   int dev = 0;
-  if (n < 0 || experts < 1 || experts > kMaxExpertsApi || cudaGetDevice(&dev) != cudaSuccess) return -1;
+  if (n < 0 || n > kMaxSize || experts < 1 || experts > kMaxExpertsApi || cudaGetDevice(&dev) != cudaSuccess) return -1;
   return static_cast<int64_t>(moe_sort_workspace_bytes(n, experts, num_sms_of(dev)));
 }
 
 NVFP4_API int nvfp4_moe_sort(const void* ids, int id_bytes, int n, int experts, int32_t* order, int32_t* slots,
                              int32_t* offsets, void* workspace, int64_t workspace_bytes, void* stream) {
   if (id_bytes != 4 && id_bytes != 8) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: ids must have 4 or 8 bytes");
-  if (n < 0) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: n=%d must not be negative", n);
+  if (n < 0 || n > kMaxSize) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: n=%d must be 0 to %lld", n, (long long)kMaxSize);
   if (experts < 1 || experts > kMaxExpertsApi)
     return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: experts=%d must be 1 to %d", experts, kMaxExpertsApi);
   if (!offsets || (n && (!ids || !order || !slots))) return fail(NVFP4_ERR_NULL, "nvfp4_moe_sort: null pointer");
@@ -543,7 +547,8 @@ static int moe_rows(const char* name, MoeRowOp op, const nvfp4_moe_args* x) {
   if (x->tokens < 0 || x->top < 0 || x->hidden < 0 || x->experts < 1 || x->experts > kMaxExpertsApi)
     return fail(NVFP4_ERR_SHAPE, "%s: tokens, top and hidden must not be negative, experts=%d must be 1 to %d", name,
                 x->experts, kMaxExpertsApi);
-  if (static_cast<int64_t>(x->tokens) * x->top > INT32_MAX) return fail(NVFP4_ERR_SHAPE, "%s: too many rows", name);
+  if (x->tokens > kMaxSize || static_cast<int64_t>(x->tokens) * x->top > kMaxSize || x->hidden > kMaxSize)
+    return fail(NVFP4_ERR_SHAPE, "%s: too large", name);
   const bool weighted = op == kMoeCombine || op == kMoeCombineBackward;
   const bool sorted_out = op == kMoeGather || op == kMoeCombineBackward;
   const bool any = x->tokens && x->hidden;   // something to write by token

@@ -72,12 +72,12 @@ def sort(ids: torch.Tensor, experts: int) -> Routing:
         _fail(f"{who}: ids must be contiguous [tokens, top], got {tuple(shape)} (strides {ids.stride()})")
     dev = _device(who, ids)
     n = shape[0] * shape[1]
-    if n >= 1 << 31:
+    if n >= (1 << 31) - (1 << 20):
         _fail(f"{who}: {n} slots do not fit 32-bit rows")
+    if not 1 <= experts <= 1024:
+        _fail(f"{who}: experts={experts} must be 1 to 1024")
     lib = _lib.load()
     need = lib.nvfp4_moe_sort_workspace(n, experts)
-    if need < 0:
-        _fail(f"{who}: experts={experts} must be 1 to 1024")
     order = ids.new_empty((n,), dtype=torch.int32)
     slots = ids.new_empty(shape, dtype=torch.int32)
     offsets = ids.new_empty((experts + 1,), dtype=torch.int32)

@@ -94,6 +94,33 @@ def test_c_refusals():
     assert rc(a=fake + 8) == 2 and rc(sfb=fake + 8) == 2 and rc(c=fake + 1) == 2 and rc(offsets=fake + 2) == 2
 
 
+@pytest.mark.parametrize("over", [2 ** 31 - 1, 2 ** 31 - 2 ** 20])
+def test_c_refuses_sizes_near_32_bits(over):
+    """The kernels round sizes up and step past them in 32-bit integers."""
+    lib, fake = _lib.load(), 1 << 20
+
+    def rc(name, struct, **kw):
+        return getattr(lib, name)(ctypes.byref(struct(**kw)))
+
+    product = dict(a=fake, b=fake, sfa=fake, sfb=fake, c=fake, experts=1, out_dtype=1, K=32)
+    assert rc("nvfp4_mx_gemm", _lib.MxGemmArgs, **product, rows=over, N=1, ldc=1) == 1
+    assert rc("nvfp4_mx_gemm", _lib.MxGemmArgs, **product, rows=1, N=over, ldc=over) == 1
+    x = dict(x=fake, packed=fake, scales=fake, dtype=1, x_rstride=64)
+    up = -(-over // 32) * 32
+    for name in ("nvfp4_mx_quantize", "nvfp4_mx_dequantize"):
+        assert rc(name, _lib.MxQuantArgs, **x, rows=1, K=min(up, 2 ** 31 - 32), experts=1) == 1
+    assert rc("nvfp4_mx_quantize", _lib.MxQuantArgs, **x, rows=1, K=over, experts=1, columns=1) == 1
+    assert rc("nvfp4_mx_quantize", _lib.MxQuantArgs, **x, rows=1, K=32, top=over, slots=fake, offsets=fake,
+              experts=4) == 1
+    assert lib.nvfp4_moe_sort(fake, 4, over, 4, fake, fake, fake, fake, 1 << 30, None) == 1
+    assert lib.nvfp4_moe_sort_workspace(over, 4) == -1
+    row = dict(in_=fake, grad=fake, weights=fake, out=fake, dweights=fake, slots=fake, offsets=fake, dtype=1, experts=4)
+    for name in ("gather", "gather_backward", "combine", "combine_backward"):
+        for sizes in [(over, 1, 1), (1, over, 1), (1, 1, over), (over, 0, 1)]:
+            tokens, top, hidden = sizes
+            assert rc("nvfp4_moe_" + name, _lib.MoeArgs, **row, tokens=tokens, top=top, hidden=hidden) == 1, (name, sizes)
+
+
 def test_struct_layout_matches_header(tmp_path):
     import os
     import shutil

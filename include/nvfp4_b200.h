@@ -202,8 +202,8 @@ int nvfp4_dual_gemm_call(const nvfp4_gemm_args* args);
  * Rows sorted by expert: offsets[experts + 1] (device memory) gives expert e
  * the rows offsets[e] .. offsets[e+1]-1.  The codes of all rows follow one
  * another; the scales of each expert begin a new 128-row block, so
- * min(rows, experts) + rows/128 blocks hold them whatever the offsets.  Rows
- * behind offsets[experts] belong to nobody: what reads rows skips them, what
+ * min(rows, experts) + rows/128 blocks hold them whatever the offsets.  Rows in
+ * front of offsets[0] or behind offsets[experts] belong to nobody: what reads rows skips them, what
  * writes rows of values writes zeros there, and the quantiser leaves them as
  * they were.  At most 1024 experts; rows, K, N, hidden and slots below 2^31 - 2^20. */
 

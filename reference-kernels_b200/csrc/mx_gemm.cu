@@ -947,9 +947,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Rows that belong to no expert (their codes stay as they were).
     if constexpr (!kCodes) {
-      if (group == 0)
-        for (int r = row_tab[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x)
+      if (group == 0) {
+        const int front = row_tab[0], others = front + p.rows - row_tab[p.experts];
+        for (int i = blockIdx.x; i < others; i += gridDim.x) {
+          const int r = i < front ? i : row_tab[p.experts] + i - front;
           for (int f = gtid; f < p.N; f += 128) c[static_cast<int64_t>(r) * p.ldc + f] = round_to<OutT>(0.f);
+        }
+      }
     }
   }
 

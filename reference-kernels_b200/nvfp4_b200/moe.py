@@ -40,7 +40,7 @@ class _Lists(NamedTuple):
 class Routing(_Lists):
     """order int32 [T*top]: the slot (token * top + choice) of each sorted row, -1 behind the last;
     slots int32 [T, top]: the sorted row of each slot, -1 where it is not routed;
-    offsets int32 [experts + 1]: each expert's first row, and the number of rows.
+    offsets int32 [experts + 1]: each expert's first row, from 0 on, and the number of rows.
 
     slots and offsets are checked once, when it is made (order is for the caller: nothing here reads it); tokens,
     top, experts and device (its CUDA index) are plain attributes."""

@@ -13,9 +13,10 @@ An operand is a pair ``(packed, scales)``:
 uint8 tensors of the same shapes are taken as well.
 
 Rows sorted by expert (``offsets``, int32 ``[experts + 1]`` on the GPU, as
-``moe.sort`` returns): ``packed`` holds all rows without gaps, ``scales`` has
-``min(rows, experts) + rows//128`` row blocks, and each expert's rows begin a
-new one.  Nothing here reads the offsets on the host.
+``moe.sort`` returns, or a part of them for some of the experts): ``packed``
+holds all rows without gaps, ``scales`` has ``min(rows, experts) + rows//128``
+row blocks, and each expert's rows begin a new one, the first expert's the
+first.  Nothing here reads the offsets on the host.
 
 Launches go to the current CUDA stream; nothing is synchronised, and everything
 can be captured into a CUDA graph.
@@ -98,8 +99,8 @@ def quantize(x: torch.Tensor, axis: int = -1, offsets: torch.Tensor | None = Non
     of 32: the operand of a product that sums over the rows, such as a weight
     gradient.
 
-    offsets: the rows are sorted by expert.  Codes of rows behind the last
-    expert's are not written."""
+    offsets: the rows are sorted by expert.  Codes of rows that no expert has
+    are not written."""
     who = "mx.quantize"
     code = _DTYPES.get(x.dtype)
     if code is None:
@@ -160,7 +161,7 @@ def _launch(name, x, packed, scales, offsets, slots, dtype, rows, k, experts, to
 def dequantize(packed: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None,
                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of an operand, [rows, K] or [E, rows, K] of ``dtype`` (exact in bf16 and fp32; fp16 rounds, and
-    overflows above 65504).  With offsets, rows behind the last expert's are zeros."""
+    overflows above 65504).  With offsets, rows that no expert has are zeros."""
     who = "mx.dequantize"
     code = _DTYPES.get(dtype)
     if code is None:
@@ -219,7 +220,7 @@ def gemm(a, sa, b, sb, offsets: torch.Tensor | None = None, out_dtype: torch.dty
     """a [rows, K] times the transpose of b [N, K] -> [rows, N], for any number of rows.
 
     With offsets, the rows are sorted by expert, b is [experts, N, K] and each row meets its expert's matrix; rows
-    behind the last expert's come out as zeros."""
+    that no expert has come out as zeros."""
     return _product("mx.gemm", a, sa, b, sb, None, None, offsets, out_dtype)
 
 

@@ -358,6 +358,29 @@ def test_offsets_that_fall_or_leave_the_rows_stay_in_bounds():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lo,hi", [(130, 200), (200, 200), (1, 7)])
+def test_rows_of_no_expert_are_zeros(lo, hi, dtype):
+    """Offsets of some of the experts: rows of others lie in front and behind."""
+    g = np.random.RandomState(9)
+    rows, n, k, experts = 300, 72, 96, 2
+    bs = [operand(n, k, g) for _ in range(experts)]
+    a = operand(rows, k, g)
+    offsets = [lo, (lo + hi) // 2, hi]
+    at, _ = mxref.scale_rows(offsets)
+    ops = on_gpu(a[0], a[1][lo:hi], at, mx.scale_blocks(rows, experts))
+    off = torch.tensor(offsets, dtype=torch.int32).cuda()
+    dirt = torch.full((rows, n), float("nan"), dtype=dtype, device="cuda")  # what the result's memory holds before
+    del dirt
+    got = mx.gemm(*ops, *weights_on_gpu(bs), offsets=off, out_dtype=dtype)
+    want = np.zeros((rows, n))
+    for s, t, w in zip(offsets[:-1], offsets[1:], bs):
+        want[s:t] = mxref.decode(a[0][s:t], a[1][s:t]) @ mxref.decode(*w).T
+    same(got, want)
+    assert _lib.device_status(True) == 0
+
+
+@pytest.mark.gpu
 def test_empty():
     b = torch.zeros((8, 32), dtype=torch.uint8, device="cuda")
     sb = torch.zeros((1, 1, 32, 4, 4), dtype=torch.uint8, device="cuda")

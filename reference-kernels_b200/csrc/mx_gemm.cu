@@ -1172,8 +1172,10 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   p.status = g.status;
   p.inject = g.inject;
   p.vec = g.out_dtype != 3 && reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && g.ldc * out_size % 16 == 0;
-  // (A TMA store ends its rows at multiples of 16 bytes only.)
-  p.tma = p.vec && static_cast<int64_t>(g.N) * out_size % 16 == 0;
+  // (A TMA store ends its rows at multiples of 16 bytes only, and its coordinates are
+  // bytes here, in 32 bits.)
+  const int64_t row_bytes = static_cast<int64_t>(g.N) * out_size;
+  p.tma = p.vec && row_bytes % 16 == 0 && row_bytes < INT32_MAX - 1024;
   const int KT = (g.K + kBK - 1) / kBK;
   const int busy = g.experts < g.rows ? g.experts : g.rows;
   const Shape shape = choose_shape(g, gate, KT, busy, num_sms);

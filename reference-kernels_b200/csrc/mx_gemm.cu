@@ -1096,28 +1096,34 @@ cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int gr
               : launch_mode<OutT, false>(g, p, smem, grid, stream, why);
 }
 
-// Tile shapes and what a K tile of theirs takes, in us, when every SM has one:
-// from 48 .. 2000 tokens with 4096x7168, 7168x2048 and 2048x4096 weights.  A tile
-// of few tokens is bound by the loads of its weights, the large ones by what an
-// SM takes from L2 (64 bytes a clock), where a pair needs half the token bytes.
+// Tile shapes, and what a K tile and the rest of a tile take, in us, when every SM
+// has one: fitted to 285 products of 1 .. 6000 tokens (up to 1024 per expert) with
+// weights of 1024x16384 .. 14336x4096, each timed in every shape, so that the shape
+// chosen is the fastest or close to it (0.6 % slower on the mean; 1.8 %, and 20 to
+// 50 for large ragged groups, without the second number).  A tile of few tokens is
+// bound by the loads of its weights, the large ones by what an SM takes from L2 (64
+// bytes a clock), where a pair needs half the token bytes; 256 tokens have one
+// accumulator, and their epilogue waits.  (Tiles of 160 and 224 tokens were never
+// faster by more than 4 %.)
 struct Shape {
   int tn, pair;
-  double k_tile_us;
+  double k_tile_us, tile_us;
 };
-constexpr Shape kShapes[] = {{32, 0, 0.18}, {64, 0, 0.205}, {128, 0, 0.28},
-                             {128, 1, 0.24}, {192, 1, 0.29}, {256, 1, 0.39}};
+constexpr Shape kShapes[] = {{32, 0, 0.17, 1.2}, {64, 0, 0.21, 0.9}, {128, 0, 0.23, 1.15},
+                             {128, 1, 0.22, 1.4}, {192, 1, 0.27, 1.25}, {256, 1, 0.34, 2.4}};
 
-// CTAs that share the K of each of at most `tiles` tiles.  One tile takes 4 + 0.18
+// CTAs that share the K of each of at most `tiles` tiles.  One tile takes 4 + 0.17
 // us per K tile on its SM; sharing K costs some 1.5 us more for the exchange and
 // divides the rest until HBM is the limit (some 65 SMs).  Measured, one token:
-// 7168x16384 18.0 -> 15.4 us with 2 CTAs, 2048x7168 9.6 -> 7.3 with 4, 1024x16384
-// 16.9 -> 9.2 with 4 and 8.4 with 8 (clusters of 8 find room for few at a time: 16
-// of them took longer than 16 of 4); 4096x4096 7.1 -> 7.4 with 2.
+// 1024x16384 14.1 -> 8.9 us with 4 CTAs and 8.0 with 8, 2048x7168 8.4 -> 7.0 with 4,
+// 7168x16384 17.2 -> 15.9 with 2; but 4096x7168 8.6 with 1, 2 and 4, 7168x12288 13.0
+// -> 13.1 with 2, 2048x2048 5.1 -> 5.7 with 4.  Clusters that find no room wait for
+// others to end: 33 of 4 (4224x7168) took 8.8 us and 34 14.1, 9 of 8 8.3 and 16 15.6.
 int k_splits(int64_t tiles, int KT, int num_sms) {
   return tiles * 8 <= num_sms / 2 && KT >= 48 ? 8
-         : tiles * 4 <= num_sms && KT >= 24   ? 4
-         : tiles * 2 <= num_sms && KT >= 32   ? 2
-                                              : 1;
+         : tiles * 5 <= num_sms && KT >= 24     ? 4
+         : tiles * 2 <= num_sms && KT >= 56     ? 2
+                                                : 1;
 }
 
 // Tiles at most, whatever the offsets.
@@ -1142,8 +1148,8 @@ Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms
     const int n_tiles = (g.N + features - 1) / features;
     const int splits = s.pair ? 1 : k_splits(most_tiles(g, s.tn, busy, n_tiles), KT, num_sms);
     const double tiles = per_expert * busy * n_tiles;
-    const double us = splits > 1 ? KT * s.k_tile_us / splits + 1.5
-                                 : std::ceil(tiles / (s.pair ? num_sms / 2 : num_sms)) * KT * s.k_tile_us;
+    const double us = splits > 1 ? KT * s.k_tile_us / splits + s.tile_us + 1.5
+                                 : std::ceil(tiles / (s.pair ? num_sms / 2 : num_sms)) * (KT * s.k_tile_us + s.tile_us);
     if (us < best_us) {
       best = s;
       best_us = us;

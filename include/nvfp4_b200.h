@@ -203,9 +203,9 @@ int nvfp4_dual_gemm_call(const nvfp4_gemm_args* args);
  * the rows offsets[e] .. offsets[e+1]-1.  The codes of all rows follow one
  * another; the scales of each expert begin a new 128-row block, so
  * min(rows, experts) + rows/128 blocks hold them whatever the offsets.  Rows in
- * front of offsets[0] or behind offsets[experts] belong to nobody: what reads rows skips them, what
- * writes rows of values writes zeros there, and the quantiser leaves them as
- * they were.  At most 1024 experts; rows, K, N, hidden and slots below 2^31 - 2^20. */
+ * front of offsets[0] or from offsets[experts] on belong to nobody: what reads
+ * rows skips them, what writes rows of values writes zeros there, and the
+ * quantiser leaves them as they were.  At most 1024 experts; rows, K, N, hidden and slots below 2^31 - 2^20. */
 
 /* x (fp16, bf16 or fp32: dtype 0, 1, 2) and its MXFP4 form.  x has `experts`
  * matrices of `rows` rows of K elements (x_estride, x_rstride elements apart),
@@ -283,7 +283,11 @@ int nvfp4_moe_sort(const void* ids, int id_bytes, int n, int experts, int32_t* o
  *                     dweights[tokens][top] = <grad[token], in[row]>   (in: ys, grad: dy)
  * Rows of `in` and `grad` are in_stride, grad_stride elements apart; out is
  * contiguous.  weights and dweights are fp32 [tokens][top]; a slot that is not
- * routed adds nothing and gets dweights 0. */
+ * routed adds nothing and gets dweights 0.  With offsets of some of the experts
+ * only, slots whose row lies outside offsets[0] .. offsets[experts] - 1 count as
+ * not routed, and rows of `out` there are zeros.  No two slots may have the same
+ * row; a row in that range that no slot has is not written.  The two sums over a
+ * token's rows take offsets == NULL too: any row counts. */
 typedef struct {
   const void* in;
   const void* grad;

@@ -10,6 +10,8 @@
 //   combine_backward  dys[row] = w[slot] * dy[token],  dw[slot] = <dy[token], ys[row]>
 // Sums are held in fp32, in the order of the slots, and rounded once; no
 // value is added with atomics, so results do not change from run to run.
+// Rows outside offsets[0] .. offsets[E] - 1 belong to nobody, whatever the slots
+// say: they are not read, and written as zeros.
 //
 // All of them are bound by memory.  The work is split by token and not by row:
 // a token's own row is then read (gather, combine_backward) or written
@@ -263,18 +265,33 @@ __host__ __device__ constexpr int in_flight(int bytes) {
   return bytes / static_cast<int>(sizeof(T) * N) < 16 ? bytes / static_cast<int>(sizeof(T) * N) : 16;
 }
 
-// Zeroes the rows of out [rows][H] that no slot has (from offsets[E] on).
+// The rows [lo, hi) that the experts have, within the `rows` that there are
+// (without offsets, which the sums over a token's rows may lack: all).
+struct Range {
+  int lo, hi;
+  __device__ __forceinline__ bool has(int row) const { return row >= lo && row < hi; }
+};
+__device__ __forceinline__ Range experts_rows(const MoeRowArgs& a) {
+  const int rows = a.tokens * a.top;
+  if (!a.offsets) return Range{0, rows};
+  const int lo = min(max(a.offsets[0], 0), rows);
+  return Range{lo, min(max(a.offsets[a.experts], lo), rows)};
+}
+
+// Zeroes the rows of out [rows][H] that no expert has, in front of the range and
+// behind it.  The slots write rows of the range alone, so that no row is written
+// by two CTAs.
 template <typename T, int N>
-__device__ __forceinline__ void zero_tail(T* out, const int* offsets, int E, int rows, int packs) {
-  const int first = min(max(offsets[E], 0), rows);
-  const int64_t n = static_cast<int64_t>(rows - first) * packs;
+__device__ __forceinline__ void zero_others(T* out, Range of, int rows, int packs) {
+  const int64_t front = static_cast<int64_t>(of.lo) * packs, own = static_cast<int64_t>(of.hi - of.lo) * packs;
+  const int64_t n = static_cast<int64_t>(rows) * packs - own;
   Pack<T, N> z;
   const float zeros[N] = {};
   z.set(zeros);
-  Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(first) * packs;
+  Pack<T, N>* const dst = reinterpret_cast<Pack<T, N>*>(out);
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-    dst[i] = z;
+    dst[i < front ? i : i + own] = z;
 }
 
 // A unit is one token and kRowThreads * kU packs of its row.
@@ -286,7 +303,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_gather_kernel(const MoeRowArg
   const int packs = a.hidden / N;
   const int per_row = (packs + kRowThreads * kU - 1) / (kRowThreads * kU);
   const int64_t units = static_cast<int64_t>(a.tokens) * per_row;
-  const int rows = a.tokens * a.top;
+  const Range of = experts_rows(a);
   T* const out = static_cast<T*>(a.out);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int t = static_cast<int>(u / per_row);
@@ -299,14 +316,14 @@ __global__ void __launch_bounds__(kRowThreads) moe_gather_kernel(const MoeRowArg
       if (p0 + i * kRowThreads < packs) v[i] = src[p0 + i * kRowThreads];
     for (int j = 0; j < a.top; ++j) {
       const int row = a.slots[static_cast<int64_t>(t) * a.top + j];
-      if (row < 0 || row >= rows) continue;
+      if (!of.has(row)) continue;
       Pack<T, N>* dst = reinterpret_cast<Pack<T, N>*>(out) + static_cast<int64_t>(row) * packs;
 #pragma unroll
       for (int i = 0; i < kU; ++i)
         if (p0 + i * kRowThreads < packs) dst[p0 + i * kRowThreads] = v[i];
     }
   }
-  zero_tail<T, N>(out, a.offsets, a.experts, rows, packs);
+  zero_others<T, N>(out, of, a.tokens * a.top, packs);
 }
 
 // combine (kWeighted) and gather_backward: a token's rows, weighted or not, added
@@ -320,7 +337,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_reduce_kernel(const MoeRowArg
   const int packs = a.hidden / N;
   const int per_row = (packs + kRowThreads * kU - 1) / (kRowThreads * kU);
   const int64_t units = static_cast<int64_t>(a.tokens) * per_row;
-  const int rows = a.tokens * a.top;
+  const Range of = experts_rows(a);
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const int t = static_cast<int>(u / per_row);
     const int p0 = static_cast<int>(u - static_cast<int64_t>(t) * per_row) * kRowThreads * kU + threadIdx.x;
@@ -345,11 +362,11 @@ __global__ void __launch_bounds__(kRowThreads) moe_reduce_kernel(const MoeRowArg
                                                                     static_cast<int64_t>(row[j]) * a.in_stride);
 #pragma unroll
         for (int i = 0; i < kU; ++i)
-          if (row[j] >= 0 && row[j] < rows && p0 + i * kRowThreads < packs) v[j][i] = src[p0 + i * kRowThreads];
+          if (of.has(row[j]) && p0 + i * kRowThreads < packs) v[j][i] = src[p0 + i * kRowThreads];
       }
 #pragma unroll
       for (int j = 0; j < kJ; ++j)
-        if (row[j] >= 0 && row[j] < rows)
+        if (of.has(row[j]))
 #pragma unroll
           for (int i = 0; i < kU; ++i)
 #pragma unroll
@@ -380,13 +397,14 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
   constexpr int kU = in_flight<T, N>(64);
   const int packs = a.hidden / N;
   const int rows = a.tokens * a.top;
+  const Range of = experts_rows(a);
   const int lane = threadIdx.x % kLanes;
   T* const out = static_cast<T*>(a.out);
   constexpr int kSlots = kRowThreads / kLanes;  // per CTA and step
   for (int64_t slot = static_cast<int64_t>(blockIdx.x) * kSlots + threadIdx.x / kLanes; slot < rows;
        slot += static_cast<int64_t>(gridDim.x) * kSlots) {
     const int row = a.slots[slot];
-    if (row < 0 || row >= rows) {  // the same for all kLanes threads
+    if (!of.has(row)) {  // the same for all kLanes threads
       if (lane == 0) a.dweights[slot] = 0.f;
       continue;
     }
@@ -437,7 +455,7 @@ __global__ void __launch_bounds__(kRowThreads) moe_combine_backward_kernel(const
       __syncthreads();
     }
   }
-  zero_tail<T, N>(out, a.offsets, a.experts, rows, packs);
+  zero_others<T, N>(out, of, rows, packs);
 }
 
 template <typename T, int N>

@@ -5,8 +5,9 @@ Each of T tokens has ``top`` slots, each with the number of an expert.
 ``sort`` gives every slot a row, by expert; numbers outside 0 .. experts-1 are
 not routed (experts of another rank: subtract this rank's first; dropped slots:
 -1).  The routing stays on the GPU: buffers of sorted rows have T*top rows
-however many are routed, and rows behind the last expert's are zeros in every
-value that a function here returns.
+however many are routed, and rows that no expert has (behind the last one's, or
+in front of the first one's where a Routing has the offsets of some of the
+experts only) are zeros in every value that a function here returns.
 
     routing = moe.sort(ids, experts)
     xs = moe.gather(x, routing)                    # [T*top, H]
@@ -40,8 +41,11 @@ class _Lists(NamedTuple):
 class Routing(_Lists):
     """order int32 [T*top]: the slot (token * top + choice) of each sorted row, -1 behind the last;
     slots int32 [T, top]: the sorted row of each slot, -1 where it is not routed;
-    offsets int32 [experts + 1]: each expert's first row, from 0 on, and the number of rows.
+    offsets int32 [experts + 1]: each expert's first row, from 0 on, and the number of rows; or the part of them for
+    some of the experts in turn, whose rows alone then count: a slot with a row outside them is as one not routed.
 
+    One made by hand gives each row of those experts to one slot: with a row in two slots the two tokens' values mix in
+    it, and a row in none is not written.
     slots and offsets are checked once, when it is made (order is for the caller: nothing here reads it); tokens,
     top, experts and device (its CUDA index) are plain attributes."""
 
@@ -185,7 +189,7 @@ def combine_backward(dy: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor, 
 
 def quantize_tokens(x: torch.Tensor, routing: Routing):
     """x [T, H] (fp16, bf16 or fp32, H % 32 == 0) -> the MXFP4 operand (packed [T*top, H/2], scales) of its sorted
-    rows: mx.quantize of gather(x), with each token quantised once.  Rows behind the last expert's are not written."""
+    rows: mx.quantize of gather(x), with each token quantised once.  Rows that no expert has are not written."""
     who = "moe.quantize_tokens"
     _, slots, offsets = routing
     tokens, top, experts = routing.tokens, routing.top, routing.experts

@@ -17,6 +17,11 @@ experts only) are zeros in every value that a function here returns.
     dys, dweights = moe.combine_backward(dy, ys, weights, routing)
     dx = moe.gather_backward(dxs, routing)
 
+Gradients are these functions; nothing here records a graph for autograd, and
+gather, combine and mlp refuse inputs that require grad while grad mode is on,
+where a result without a graph would lose the gradient.  Call them under
+torch.no_grad(), as the forward of a torch.autograd.Function is.
+
 Sums are in fp32, in the order of the slots, so that results are the same on
 every run.  Launches go to the current CUDA stream; nothing is synchronised, and
 everything can be captured into a CUDA graph.
@@ -105,6 +110,14 @@ def _on(who: str, routing: Routing, t: torch.Tensor, *others) -> int:
     return dev
 
 
+def _no_graph(who: str, *inputs) -> None:
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t.requires_grad:
+                _fail(f"{who}: an input requires grad, but no graph is recorded; call under torch.no_grad() "
+                      f"(moe.gather_backward and moe.combine_backward are the gradients)")
+
+
 def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int):
     """(dtype code, hidden, row stride) of t [rows, hidden]."""
     code = _DTYPES.get(t.dtype)
@@ -142,6 +155,7 @@ def gather(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     who = "moe.gather"
     tokens = routing.tokens
     code, h, stride = _check_matrix(who, "x", x, tokens)
+    _no_graph(who, x)
     dev = _on(who, routing, x)
     xs = x.new_empty((tokens * routing.top, h))
     _rows("nvfp4_moe_gather", routing, x, None, None, xs, None, code, h, stride, 0, dev)
@@ -165,6 +179,7 @@ def combine(ys: torch.Tensor, weights: torch.Tensor, routing: Routing) -> torch.
     tokens = routing.tokens
     code, h, stride = _check_matrix(who, "ys", ys, tokens * routing.top)
     _check_weights(who, weights, routing)
+    _no_graph(who, ys, weights)
     dev = _on(who, routing, ys, weights)
     y = ys.new_empty((tokens, h))
     _rows("nvfp4_moe_combine", routing, ys, None, weights, y, None, code, h, stride, 0, dev)
@@ -213,6 +228,7 @@ def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, dow
     (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  x and the result are fp16, bf16 or
     fp32; the tokens are quantised to MXFP4 as they are sorted, the gated values in the product's epilogue, and the
     down projection's rows have x's type.  Five launches (six for more than 32768 slots), no synchronisation."""
+    _no_graph("moe.mlp", x, weights)
     if gate[0].dim() != 3:
         _fail(f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
     routing = sort(ids, gate[0].shape[0])

@@ -20,6 +20,10 @@ first.  Nothing here reads the offsets on the host.
 
 Launches go to the current CUDA stream; nothing is synchronised, and everything
 can be captured into a CUDA graph.
+
+Codes carry no gradient, like the integers that torch converts to: quantize of a
+tensor that requires grad is a constant to autograd, and so is what is computed
+from it.  A gradient is a product of its own (quantize, axis=0).
 """
 from __future__ import annotations
 

@@ -34,6 +34,8 @@ from .inputs import FP4X2
 from .ops import _CHECK_STATUS, _post
 
 E8M0 = torch.float8_e8m0fnu
+_CODES = (FP4X2, torch.uint8)
+_SCALES = (E8M0, torch.uint8)
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -75,7 +77,7 @@ def scale_blocks(rows: int, experts: int | None = None) -> int:
 def _check_operand(who: str, packed: torch.Tensor, scales: torch.Tensor, dim: int, experts: int | None = None):
     """The shape of an operand's packed tensor; ``dim``: its dimensions; ``experts``: rows are sorted by expert."""
     shape = packed.shape
-    if len(shape) != dim or packed.element_size() != 1 or not packed.is_contiguous():
+    if len(shape) != dim or packed.dtype not in _CODES or not packed.is_contiguous():
         _fail(f"{who}: codes must be contiguous float4_e2m1fn_x2 or uint8 of {dim} dimensions, "
               f"got {packed.dtype} {tuple(shape)} (strides {packed.stride()})")
     k2 = shape[-1]
@@ -84,7 +86,7 @@ def _check_operand(who: str, packed: torch.Tensor, scales: torch.Tensor, dim: in
     want = (scale_blocks(shape[-2], experts), -(-k2 // 64), 32, 4, 4)
     if dim == 3:
         want = (shape[0], *want)
-    if scales.shape != want or scales.element_size() != 1 or not scales.is_contiguous():
+    if scales.shape != want or scales.dtype not in _SCALES or not scales.is_contiguous():
         _fail(f"{who}: scales must be contiguous float8_e8m0fnu or uint8 {want}, "
               f"got {scales.dtype} {tuple(scales.shape)} (strides {scales.stride()})")
     return shape

@@ -61,7 +61,7 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w) {
 template <typename T>
 struct Block {
   static constexpr int kWords = 8 * sizeof(T);
-  uint32_t w[kWords];
+  alignas(16) uint32_t w[kWords];  // (loaded in 16-byte pieces)
 
   // kAlign: bytes that the address is a multiple of, 32 or 16.
   template <int kAlign>
@@ -243,7 +243,10 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_kernel(const MxQuantArgs
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) mx_quantize_columns_kernel(const MxQuantArgs a) {
   __shared__ uint4 codes[64][kWarps + 1];
-  __shared__ uint8_t sc[64][kWarps];
+  struct alignas(4) Scales {  // of a column, stored to memory as words
+    uint8_t code[kWarps];
+  };
+  __shared__ Scales sc[64];
   if (threadIdx.x == 0) pdl_allow_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_columns_kernel(const MxQ
     for (int i = 0; i < 32; ++i) reinterpret_cast<T*>(b.w)[i] = v[i].v[h];
     const uint32_t code = scale_code(b.amax_bits());
     codes[2 * lane + h][warp] = b.codes(code);
-    sc[2 * lane + h][warp] = r0 < Kt ? static_cast<uint8_t>(code) : 0;
+    sc[2 * lane + h].code[warp] = r0 < Kt ? static_cast<uint8_t>(code) : 0;
   }
   __syncthreads();
   const int k0 = blockIdx.y * 256;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kThreads) mx_quantize_columns_kernel(const MxQ
     const int col = threadIdx.x >> 1, j = threadIdx.x & 1;
     if (c0 + col < C && (k0 >> 7) + j < K128)
       *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.scales) + mx_scale_word(c0 + col, (k0 >> 7) + j, K128)) =
-          reinterpret_cast<const uint32_t*>(sc[col])[j];
+          reinterpret_cast<const uint32_t*>(sc[col].code)[j];
   }
 }
 

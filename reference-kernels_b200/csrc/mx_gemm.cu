@@ -1112,6 +1112,30 @@ struct Shape {
 constexpr Shape kShapes[] = {{32, 0, 0.17, 1.2}, {64, 0, 0.21, 0.9}, {128, 0, 0.23, 1.15},
                              {128, 1, 0.22, 1.4}, {192, 1, 0.27, 1.25}, {256, 1, 0.34, 2.4}};
 
+// 128-row scale blocks that a tile of tn tokens can touch: an expert's tiles begin
+// at multiples of tn, a multiple of 32, so at up to four places within a block.
+constexpr int tile_scale_blocks(int tn) {
+  int most = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int blocks = ((i * tn % 128) + tn - 1) / 128 + 1;
+    most = blocks > most ? blocks : most;
+  }
+  return most;
+}
+// TMEM columns of the token scales of 128 K columns.
+constexpr int tile_scale_cols(int tn) { return tn <= 128 ? 4 : tn / 32; }
+// What the kernel takes for granted of a shape: the scale writers hold the words of
+// two scale blocks and store 4, 6 or 8 of them (224 tokens that begin at row 96 of a
+// block touch three, and have 7).
+constexpr bool shapes_fit() {
+  for (const Shape& s : kShapes) {
+    const int cols = tile_scale_cols(s.tn);
+    if (s.tn % 32 || s.tn > 256 || tile_scale_blocks(s.tn) > 2 || (cols != 4 && cols != 6 && cols != 8)) return false;
+  }
+  return true;
+}
+static_assert(shapes_fit(), "a tile shape that the kernel is not made for");
+
 // CTAs that share the K of each of at most `tiles` tiles.  One tile takes 4 + 0.17
 // us per K tile on its SM; sharing K costs some 1.5 us more for the exchange and
 // divides the rest until HBM is the limit (some 65 SMs).  Measured, one token:
@@ -1190,9 +1214,9 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   const int features = (gate ? 64 : 128) * (p.pair ? 2 : 1);
   p.n_tiles = (g.N + features - 1) / features;
   const int x_rows = p.pair ? p.tn / 2 : p.tn;  // token rows in a CTA's shared memory
-  p.nblk = p.tn <= 128 ? 1 : 2;
+  p.nblk = tile_scale_blocks(p.tn);
   p.acc_bufs = p.tn <= 192 ? 2 : 1;
-  p.x_cols = p.tn <= 128 ? 4 : p.tn / 32;
+  p.x_cols = tile_scale_cols(p.tn);
   p.sf_cols = 8 + 2 * p.x_cols;
   const int64_t exact = most_tiles(g, p.tn, busy, p.n_tiles);
   p.splits = p.pair ? 1 : k_splits(exact, KT, num_sms);

@@ -263,6 +263,13 @@ typedef struct {
 
 int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* args);
 
+/* How nvfp4_mx_gemm shares the work of such a call on a GPU of num_sms SMs: the
+ * tokens of a tile, the CTAs that share a tile (1, 2) and the CTAs that share its K.
+ * Launches nothing and needs no GPU; of the pointers only whether b2 and offsets
+ * are null matters. */
+int nvfp4_mx_gemm_shape(const nvfp4_mx_gemm_args* args, int num_sms, int32_t* tokens, int32_t* ctas,
+                        int32_t* k_splits);
+
 /* Sorts n slots by expert, stably: ids[n] (int32 or int64: id_bytes 4, 8);
  * an id outside 0 .. experts-1 is not routed.
  *   order[n]           the slot of each sorted row, -1 behind the last

@@ -480,8 +480,8 @@ NVFP4_API int nvfp4_mx_dequantize(const nvfp4_mx_quant_args* x) {
   return NVFP4_OK;
 }
 
-NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
-  const char* name = "nvfp4_mx_gemm";
+// The checks of a product's sizes.
+static int mx_gemm_sizes(const char* name, const nvfp4_mx_gemm_args* x) {
   if (!x) return fail(NVFP4_ERR_NULL, "%s: null argument block", name);
   if (x->out_dtype < 0 || x->out_dtype > 3)
     return fail(NVFP4_ERR_SHAPE, "%s: out_dtype must be 0 (fp16), 1 (bf16), 2 (fp32) or 3 (MXFP4)", name);
@@ -498,6 +498,14 @@ NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
   if (x->rows > kMaxSize || x->N > kMaxSize || x->K > (1 << 24) ||
       (static_cast<int64_t>(x->rows) / 32 + x->experts) * ((static_cast<int64_t>(x->N) + 63) / 64) > kMaxSize)
     return fail(NVFP4_ERR_SHAPE, "%s: too large", name);
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
+  const char* name = "nvfp4_mx_gemm";
+  const int rc = mx_gemm_sizes(name, x);
+  if (rc) return rc;
+  const bool codes = x->out_dtype == 3;
   if (x->rows == 0) return NVFP4_OK;
   if (!x->a || !x->b || !x->sfa || !x->sfb || !x->c || !x->b2 != !x->sfb2 || (codes && !x->c_scales))
     return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
@@ -511,6 +519,27 @@ NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
   const char* why = nullptr;
   const cudaError_t e = launch_mx_gemm(g, num_sms_of(dev), static_cast<cudaStream_t>(x->stream), &why);
   if (e != cudaSuccess) return fail(NVFP4_ERR_CUDA, "%s: %s", name, why ? why : cudaGetErrorString(e));
+  return NVFP4_OK;
+}
+
+NVFP4_API int nvfp4_mx_gemm_shape(const nvfp4_mx_gemm_args* x, int num_sms, int32_t* tokens, int32_t* ctas,
+                                  int32_t* k_splits) {
+  const char* name = "nvfp4_mx_gemm_shape";
+  const int rc = mx_gemm_sizes(name, x);
+  if (rc) return rc;
+  if (x->rows == 0 || num_sms < 2) return fail(NVFP4_ERR_SHAPE, "%s: rows must be positive, num_sms 2 or more", name);
+  if (!tokens || !ctas || !k_splits) return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
+  MxGemmArgs g{};
+  g.b2 = x->b2;
+  g.offsets = x->offsets;
+  g.rows = x->rows;
+  g.N = x->N;
+  g.K = x->K;
+  g.experts = x->experts;
+  const MxGemmShape shape = mx_gemm_shape(g, num_sms);
+  *tokens = shape.tn;
+  *ctas = shape.pair ? 2 : 1;
+  *k_splits = shape.splits;
   return NVFP4_OK;
 }
 

@@ -169,6 +169,11 @@ struct MxGemmArgs {
   int* status;
   int inject;
 };
+// Tokens of a tile, whether two CTAs share it, and CTAs that share its K.
+struct MxGemmShape {
+  int tn, pair, splits;
+};
+MxGemmShape mx_gemm_shape(const MxGemmArgs& g, int num_sms);
 cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why);
 
 // Tokens sorted by expert and back (moe.cu).

@@ -1150,6 +1150,12 @@ int k_splits(int64_t tiles, int KT, int num_sms) {
                                                 : 1;
 }
 
+// Output features of a tile.
+int tile_features(bool gate, int pair) { return (gate ? 64 : 128) * (pair ? 2 : 1); }
+
+// Experts that can have a row.
+int busy_experts(const MxGemmArgs& g) { return g.experts < g.rows ? g.experts : g.rows; }
+
 // Tiles at most, whatever the offsets.
 int64_t most_tiles(const MxGemmArgs& g, int tn, int busy, int n_tiles) {
   return g.offsets ? (static_cast<int64_t>(g.rows) / tn + busy) * n_tiles
@@ -1163,7 +1169,7 @@ Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms
   Shape best = kShapes[0];
   double best_us = 1e30;
   for (const Shape& s : kShapes) {
-    const int features = (gate ? 64 : 128) * (s.pair ? 2 : 1);
+    const int features = tile_features(gate, s.pair);
     double per_expert = 0;
     if (g.offsets)
       for (const double f : {0.6, 0.8, 1.0, 1.2, 1.5}) per_expert += std::ceil(f * mean / s.tn) / 5;
@@ -1183,6 +1189,14 @@ Shape choose_shape(const MxGemmArgs& g, bool gate, int KT, int busy, int num_sms
 }
 
 }  // namespace
+
+MxGemmShape mx_gemm_shape(const MxGemmArgs& g, int num_sms) {
+  const bool gate = g.b2 != nullptr;
+  const int KT = (g.K + kBK - 1) / kBK, busy = busy_experts(g);
+  const Shape s = choose_shape(g, gate, KT, busy, num_sms);
+  const int features = tile_features(gate, s.pair), n_tiles = (g.N + features - 1) / features;
+  return MxGemmShape{s.tn, s.pair, s.pair ? 1 : k_splits(most_tiles(g, s.tn, busy, n_tiles), KT, num_sms)};
+}
 
 cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream, const char** why) {
   const bool gate = g.b2 != nullptr;
@@ -1206,20 +1220,18 @@ cudaError_t launch_mx_gemm(const MxGemmArgs& g, int num_sms, cudaStream_t stream
   // bytes here, in 32 bits.)
   const int64_t row_bytes = static_cast<int64_t>(g.N) * out_size;
   p.tma = p.vec && row_bytes % 16 == 0 && row_bytes < INT32_MAX - 1024;
-  const int KT = (g.K + kBK - 1) / kBK;
-  const int busy = g.experts < g.rows ? g.experts : g.rows;
-  const Shape shape = choose_shape(g, gate, KT, busy, num_sms);
+  const MxGemmShape shape = mx_gemm_shape(g, num_sms);
   p.tn = shape.tn;
   p.pair = shape.pair;
-  const int features = (gate ? 64 : 128) * (p.pair ? 2 : 1);
+  p.splits = shape.splits;
+  const int features = tile_features(gate, shape.pair);
   p.n_tiles = (g.N + features - 1) / features;
   const int x_rows = p.pair ? p.tn / 2 : p.tn;  // token rows in a CTA's shared memory
   p.nblk = tile_scale_blocks(p.tn);
   p.acc_bufs = p.tn <= 192 ? 2 : 1;
   p.x_cols = tile_scale_cols(p.tn);
   p.sf_cols = 8 + 2 * p.x_cols;
-  const int64_t exact = most_tiles(g, p.tn, busy, p.n_tiles);
-  p.splits = p.pair ? 1 : k_splits(exact, KT, num_sms);
+  const int64_t exact = most_tiles(g, p.tn, busy_experts(g), p.n_tiles);
   // Stages: what shared memory and TMEM hold.
   const size_t fixed = fixed_smem(out_size, gate, g.experts) + (p.splits > 1 ? sums_bytes(p.tn, p.splits) : 0);
   const size_t stage = kABytes + x_rows * kBKBytes + ((gate ? 2 : 1) + p.nblk) * kSfBytes;

@@ -32,6 +32,7 @@ EXPORTS = (
     "nvfp4_mx_quantize",
     "nvfp4_mx_dequantize",
     "nvfp4_mx_gemm",
+    "nvfp4_mx_gemm_shape",
     "nvfp4_moe_sort_workspace",
     "nvfp4_moe_sort",
     "nvfp4_moe_gather",
@@ -145,6 +146,8 @@ def load() -> ctypes.CDLL:
                  "nvfp4_moe_gather_backward", "nvfp4_moe_combine", "nvfp4_moe_combine_backward"):
         getattr(lib, name).restype = _I
         getattr(lib, name).argtypes = [_P]
+    lib.nvfp4_mx_gemm_shape.restype = _I
+    lib.nvfp4_mx_gemm_shape.argtypes = [_P, _I, _P, _P, _P]
     lib.nvfp4_moe_sort_workspace.restype = _L
     lib.nvfp4_moe_sort_workspace.argtypes = [_I, _I]
     lib.nvfp4_moe_sort.restype = _I

@@ -489,7 +489,8 @@ static int mx_gemm_sizes(const char* name, const nvfp4_mx_gemm_args* x) {
   if (x->rows < 0 || x->N <= 0 || x->K <= 0 || x->experts < 1)
     return fail(NVFP4_ERR_SHAPE, "%s: rows must not be negative; N, K and experts must be positive", name);
   if (x->K % 32) return fail(NVFP4_ERR_SHAPE, "%s: K=%d must be a multiple of 32", name, x->K);
-  if (x->experts > kMaxExpertsApi) return fail(NVFP4_ERR_SHAPE, "%s: %d experts, at most %d", name, x->experts, kMaxExpertsApi);
+  if (x->experts > kMaxExpertsApi)
+    return fail(NVFP4_ERR_SHAPE, "%s: %d experts, at most %d", name, x->experts, kMaxExpertsApi);
   if (x->experts != 1 && !x->offsets) return fail(NVFP4_ERR_NULL, "%s: several experts need offsets", name);
   if (!codes && x->ldc < x->N)
     return fail(NVFP4_ERR_SHAPE, "%s: ldc=%lld < N=%d", name, (long long)x->ldc, x->N);
@@ -510,7 +511,8 @@ NVFP4_API int nvfp4_mx_gemm(const nvfp4_mx_gemm_args* x) {
   if (!x->a || !x->b || !x->sfa || !x->sfb || !x->c || !x->b2 != !x->sfb2 || (codes && !x->c_scales))
     return fail(NVFP4_ERR_NULL, "%s: null pointer", name);
   if (!aligned(x->a, 16) || !aligned(x->b, 16) || !aligned(x->b2, 16) || !aligned(x->sfa, 16) || !aligned(x->sfb, 16) ||
-      !aligned(x->sfb2, 16) || !aligned(x->c, codes ? 16 : dtype_size(x->out_dtype)) || !aligned(x->c_scales, 16) || !aligned(x->offsets, 4))
+      !aligned(x->sfb2, 16) || !aligned(x->c, codes ? 16 : dtype_size(x->out_dtype)) || !aligned(x->c_scales, 16) ||
+      !aligned(x->offsets, 4))
     return fail(NVFP4_ERR_ALIGN, "%s: codes and scales need 16-byte alignment, c that of its type", name);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4_ERR_DEVICE, "%s: no CUDA device", name);
@@ -552,7 +554,8 @@ NVFP4_API int64_t nvfp4_moe_sort_workspace(int n, int experts) {
 NVFP4_API int nvfp4_moe_sort(const void* ids, int id_bytes, int n, int experts, int32_t* order, int32_t* slots,
                              int32_t* offsets, void* workspace, int64_t workspace_bytes, void* stream) {
   if (id_bytes != 4 && id_bytes != 8) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: ids must have 4 or 8 bytes");
-  if (n < 0 || n > kMaxSize) return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: n=%d must be 0 to %lld", n, (long long)kMaxSize);
+  if (n < 0 || n > kMaxSize)
+    return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: n=%d must be 0 to %lld", n, (long long)kMaxSize);
   if (experts < 1 || experts > kMaxExpertsApi)
     return fail(NVFP4_ERR_SHAPE, "nvfp4_moe_sort: experts=%d must be 1 to %d", experts, kMaxExpertsApi);
   if (!offsets || (n && (!ids || !order || !slots))) return fail(NVFP4_ERR_NULL, "nvfp4_moe_sort: null pointer");

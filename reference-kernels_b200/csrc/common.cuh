@@ -314,6 +314,9 @@ __device__ __forceinline__ void set_status(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }
 
+// x / (1 + exp(-x)) * y in fp32, with the fast exponential and quotient: off by some
+// (6 + 1.2 |x|) 2^-23 of the value, which 16-bit results do not show; 0 below x = -87,
+// where exp(-x) is past the quotient's range and the silu is under 1e-35.
 __device__ __forceinline__ float silu_mul(float x, float y) {
   return __fdividef(x, 1.0f + __expf(-x)) * y;
 }

@@ -30,8 +30,9 @@ namespace {
 
 // ------------------------------------------------------------------ sort
 // A stable counting sort.  A CTA takes a run of slots and each of its 32 warps
-// a part of that run; within a warp 32 slots at a time are ranked by ballots.  hist[warp][expert] in shared memory first counts, then (after
-// sums over the warps, the CTAs and the experts) holds the next free row.
+// a part of that run; within a warp 32 slots at a time are ranked by ballots.
+// hist[warp][expert] in shared memory first counts, then (after sums over the warps,
+// the CTAs and the experts) holds the next free row.
 // One CTA does short lists, a cluster of eight longer ones, whose CTAs read one
 // another's counts from distributed shared memory.  Lists that keep a cluster's
 // warps busy for long take a second launch, before it, that counts each CTA's run
@@ -498,7 +499,8 @@ cudaError_t launch_type(MoeRowOp op, const MoeRowArgs& a, int num_sms, cudaStrea
 template <typename K>
 cudaError_t allow_smem(K kernel, size_t smem) {
   if (smem <= 40 * 1024) return cudaSuccess;  // (with the static part under the default 48 KB)
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortWarps * kMaxExperts * sizeof(int));
+  constexpr int kMost = kSortWarps * kMaxExperts * static_cast<int>(sizeof(int));
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
 }
 
 template <typename Id>

@@ -24,17 +24,20 @@
 //                  tcgen05.cp would take tensor-pipe time).  A token tile that
 //                  begins inside a block of 128 takes its words from the block's
 //                  middle on.
-// Over 128 tokens, pairs of CTAs (cta_group::2): 256 weight rows, each CTA with its
-// own half of them and of the tokens, which halves the token bytes per SM.
+// Tiles of 128 to 256 tokens may be shared by a pair of CTAs (cta_group::2): 256
+// weight rows, each CTA with its own half of them and of the tokens, which halves the
+// token bytes per SM.  choose_shape weighs them with the tiles of one CTA.
 //
 // What bounds it, on B200: few tokens by HBM -- 32 tokens over 64 experts, gated,
 // 2048x4096: 76 us for 0.56 GB, 7.4 TB/s, above the 6.6 TB/s of a copy; one token
 // through 7168x16384 15.2 us, 9.5 of them traffic, the rest set-up, the first
-// loads' latency and the exchange of partial sums.  Many tokens by what an SM
-// takes from L2: a pair's 192-token tile needs 31 KB per 384 cycles of MMA, and
-// 57 bytes a clock arrive of the 64 that an SM's port has -- 1000x7168x16384 47 us
-// (5.0 PFLOP/s), 8192x7168x4096 93 us, 8192x7168x16384 327 us (5.9 PFLOP/s, 0.88
-// of 4 x the measured bf16 rate).  Over seconds the power cap takes 15 % of that.
+// loads' latency and the exchange of partial sums.  Many tokens by nothing alone:
+// 8192x7168x4096 (93 us, 5.1 PFLOP/s) has the tensor pipe busy for 74 % of the time,
+// takes 55 bytes a clock and SM from L2 (12.9 TB/s, 43 % of what the counter has as
+// its peak) and has the clock down to 1.57 GHz.  What a tile costs beside its K tiles
+// (kShapes) is 22 % of it at K = 4096; 8192x7168x16384 takes 327 us (5.9 PFLOP/s, 0.88
+// of 4 x the measured bf16 rate).  1000x7168x16384 (47 us, 5.0 PFLOP/s) has 112 tiles
+// for 74 pairs.  Over seconds the power cap takes 15 % of these.
 // The offsets are read on the device: every CTA builds the table of the experts'
 // rows, scale blocks and tiles in shared memory and walks the same tile list, so
 // the host never waits for a routing.
@@ -210,8 +213,8 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bulk_load_u32(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
                                               uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
-          dst),
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;" ::"r"(dst),
       "l"(src), "r"(bytes), "r"(bar), "l"(policy)
       : "memory");
 }
@@ -462,10 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = __shfl_sync(0xffffffffu, total, 0);
       const uint64_t keep = policy_evict_last(), once = policy_evict_first();
       const int P = p.producers;
-      int e = 0, stage = producer, ahead = producer;  // ahead: this producer's next K tile, counted from the tile's first
+      int e = 0, stage = producer;
+      int ahead = producer;  // this producer's next K tile, counted from the tile's first
       uint32_t phase = 1;
       const int wblocks = (p.N + 127) >> 7;
-      const uint32_t stages0 = __shfl_sync(0xffffffffu, smem_u32(smem), 0), sf0 = __shfl_sync(0xffffffffu, smem_u32(sfbuf), 0);
+      const uint32_t stages0 = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const uint32_t sf0 = __shfl_sync(0xffffffffu, smem_u32(sfbuf), 0);
       const uint32_t full0 = __shfl_sync(0xffffffffu, smem_u32(full), 0), sf_full0 = full0 + 16 * S;
       bool ok = true;
       for (int t = t0; t < tiles && ok; t += step) {
@@ -1077,8 +1082,9 @@ cudaError_t launch(const MxGemmArgs& g, const Params& p, size_t smem, int grid, 
     *why = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, kMode == kSplitK ? p.splits : kMode == kPairs ? 2 : 1, tw, kGate ? tw2 : tw, tx,
-                    txs, p.tma ? tc : tx, p);
+  const int cluster = kMode == kSplitK ? p.splits : kMode == kPairs ? 2 : 1;
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, stream, cluster, tw, kGate ? tw2 : tw, tx, txs,
+                    p.tma ? tc : tx, p);
 }
 
 template <typename OutT, bool kGate>
@@ -1099,11 +1105,10 @@ cudaError_t launch_out(const MxGemmArgs& g, const Params& p, size_t smem, int gr
 // Tile shapes, and what a K tile and the rest of a tile take, in us, when every SM
 // has one: fitted to 285 products of 1 .. 6000 tokens (up to 1024 per expert) with
 // weights of 1024x16384 .. 14336x4096, each timed in every shape, so that the shape
-// chosen is the fastest or close to it (0.6 % slower on the mean; 1.8 %, and 20 to
-// 50 for large ragged groups, without the second number).  A tile of few tokens is
-// bound by the loads of its weights, the large ones by what an SM takes from L2 (64
-// bytes a clock), where a pair needs half the token bytes; 256 tokens have one
-// accumulator, and their epilogue waits.  (Tiles of 160 and 224 tokens were never
+// chosen is the fastest or close to it (0.5 % slower on the mean, 7 % at worst).  A
+// tile of few tokens is bound by the loads of its weights; of the large ones a pair's
+// need half the token bytes; 256 tokens have one accumulator, and their epilogue
+// waits.  (Tiles of 160 and 224 tokens were never
 // faster by more than 4 %.)
 struct Shape {
   int tn, pair;
@@ -1136,9 +1141,10 @@ constexpr bool shapes_fit() {
 }
 static_assert(shapes_fit(), "a tile shape that the kernel is not made for");
 
-// CTAs that share the K of each of at most `tiles` tiles.  One tile takes 4 + 0.17
-// us per K tile on its SM; sharing K costs some 1.5 us more for the exchange and
-// divides the rest until HBM is the limit (some 65 SMs).  Measured, one token:
+// CTAs that share the K of each of at most `tiles` tiles.  A call of one tile per SM
+// takes 4 + 0.17 us per K tile (launch, set-up and first loads are in the 4; kShapes
+// has what a tile adds to a round); sharing K costs some 1.5 us more for the exchange
+// and divides the rest until HBM is the limit (some 65 SMs).  Measured, one token:
 // 1024x16384 14.1 -> 8.9 us with 4 CTAs and 8.0 with 8, 2048x7168 8.4 -> 7.0 with 4,
 // 7168x16384 17.2 -> 15.9 with 2; but 4096x7168 8.6 with 1, 2 and 4, 7168x12288 13.0
 // -> 13.1 with 2, 2048x2048 5.1 -> 5.7 with 4.  Clusters that find no room wait for

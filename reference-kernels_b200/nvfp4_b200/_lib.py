@@ -75,8 +75,9 @@ class MxQuantArgs(ctypes.Structure):
 class MxGemmArgs(ctypes.Structure):
     """nvfp4_mx_gemm_args of include/nvfp4_b200.h."""
     _fields_ = [("a", _P), ("b", _P), ("b2", _P), ("sfa", _P), ("sfb", _P), ("sfb2", _P), ("c", _P),
-                ("c_scales", _P), ("offsets", _P), ("rows", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("experts", ctypes.c_int32),
-                ("out_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("ldc", _L), ("stream", _P)]
+                ("c_scales", _P), ("offsets", _P), ("rows", ctypes.c_int32), ("N", ctypes.c_int32),
+                ("K", ctypes.c_int32), ("experts", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("ldc", _L), ("stream", _P)]
 
 
 class MoeArgs(ctypes.Structure):

@@ -110,12 +110,11 @@ def _on(who: str, routing: Routing, t: torch.Tensor, *others) -> int:
     return dev
 
 
-def _no_graph(who: str, *inputs) -> None:
+def _no_graph(who: str) -> None:
+    """For inputs of which one requires grad."""
     if torch.is_grad_enabled():
-        for t in inputs:
-            if t.requires_grad:
-                _fail(f"{who}: an input requires grad, but no graph is recorded; call under torch.no_grad() "
-                      f"(moe.gather_backward and moe.combine_backward are the gradients)")
+        _fail(f"{who}: an input requires grad, but no graph is recorded; call under torch.no_grad() "
+              f"(moe.gather_backward and moe.combine_backward are the gradients)")
 
 
 def _check_matrix(who: str, name: str, t: torch.Tensor, rows: int):
@@ -155,7 +154,8 @@ def gather(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     who = "moe.gather"
     tokens = routing.tokens
     code, h, stride = _check_matrix(who, "x", x, tokens)
-    _no_graph(who, x)
+    if x.requires_grad:
+        _no_graph(who)
     dev = _on(who, routing, x)
     xs = x.new_empty((tokens * routing.top, h))
     _rows("nvfp4_moe_gather", routing, x, None, None, xs, None, code, h, stride, 0, dev)
@@ -179,7 +179,8 @@ def combine(ys: torch.Tensor, weights: torch.Tensor, routing: Routing) -> torch.
     tokens = routing.tokens
     code, h, stride = _check_matrix(who, "ys", ys, tokens * routing.top)
     _check_weights(who, weights, routing)
-    _no_graph(who, ys, weights)
+    if ys.requires_grad or weights.requires_grad:
+        _no_graph(who)
     dev = _on(who, routing, ys, weights)
     y = ys.new_empty((tokens, h))
     _rows("nvfp4_moe_combine", routing, ys, None, weights, y, None, code, h, stride, 0, dev)
@@ -222,13 +223,15 @@ def quantize_tokens(x: torch.Tensor, routing: Routing):
 
 
 def mlp(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate, up, down) -> torch.Tensor:
-    """The experts' MLP on x [T, H]: y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])), e = ids[t, j].
+    """The experts' MLP on x [T, H]: y[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
+    e = ids[t, j].
 
     gate, up: operands (packed, scales) of [experts, N, H] weights, down of [experts, H, N], as mx.quantize makes them
     (H and N multiples of 32); ids [T, top] as for sort, weights fp32 [T, top].  x and the result are fp16, bf16 or
     fp32; the tokens are quantised to MXFP4 as they are sorted, the gated values in the product's epilogue, and the
     down projection's rows have x's type.  Five launches (six for more than 32768 slots), no synchronisation."""
-    _no_graph("moe.mlp", x, weights)
+    if x.requires_grad or weights.requires_grad:
+        _no_graph("moe.mlp")
     if gate[0].dim() != 3:
         _fail(f"moe.mlp: gate must be weights [experts, N, H/2], got {tuple(gate[0].shape)}")
     routing = sort(ids, gate[0].shape[0])
